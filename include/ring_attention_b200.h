@@ -252,6 +252,130 @@ int ring_attention_chunked_fwd_static(const void* q, const void* k, const void* 
  */
 int ring_static_status(int* status_out, void* stream);
 
+/* ------------------------------------------------------------------------------------------------ paged K/V cache
+ * Serving operators over a paged K/V cache: what a sequence needs after its prompt went through the forward above.
+ * No counterpart in the reference (a forward over whole shards only).
+ *
+ * Cache.  K and V live in `num_pages` pages of `page_size` places per K/V head.  A place is a row of `dim` contiguous
+ * elements; pages, heads and places may be laid out in any order (strides in elements, multiples of 8, bases 16-byte
+ * aligned), so both [pages, kv_heads, page_size, dim] and [pages, page_size, kv_heads, dim] are served.  page_size is a
+ * power of two >= 8.
+ * Sequences.  page_table[b * table_stride + i] (device, int32) names the page holding places [i, i + 1) * page_size of
+ * sequence b; kv_lens[b] (device, int32) is its length in places INCLUDING this step's new tokens.  An id outside
+ * [0, num_pages) holds no places: they are seen by nobody and nothing is written there.  Lengths are clamped to
+ * [0, max_pages * page_size].
+ * New tokens.  `tokens` rows are packed sequence after sequence: rows cu_seqlens[b] .. cu_seqlens[b + 1] (device, int32,
+ * batch + 1 entries, ascending) belong to sequence b; with cu_seqlens == NULL every sequence brings tokens / batch of them.
+ * Token i of the n_b of sequence b has place kv_lens[b] - n_b + i.  Rows outside every sequence are neither read nor written.
+ * max_new is an upper bound on n_b, used to choose a kernel (0: tokens); results stay right if it is too small.
+ * The lengths stay on the device: no call waits for the GPU, allocates or keeps anything between calls, so calls may be captured
+ * into graphs and overlap (each with a workspace of its own).  As everywhere in this library, the first call on a
+ * device does its one-time set-up; make it before any stream capture.  All of it runs on the current device.
+ */
+typedef struct Ring_paged_params {
+    /* cache */
+    void* k_cache;
+    void* v_cache;
+    int64_t k_page_stride, k_head_stride, k_place_stride;
+    int64_t v_page_stride, v_head_stride, v_place_stride;
+    int num_pages, page_size, kv_heads, dim;
+    /* sequences */
+    const int* page_table;
+    int64_t table_stride;
+    int max_pages; /* entries of a page_table row */
+    int batch;
+    const int* kv_lens;
+    const int* cu_seqlens; /* or NULL */
+    int tokens;
+    int max_new;
+    /* queries: attention and weights.  q, out [tokens, heads, dim] by strides, lse [tokens, heads] fp32 contiguous */
+    const void* q;
+    int64_t q_token_stride, q_head_stride;
+    int heads; /* a multiple of kv_heads: query head x reads K/V head x / (heads / kv_heads) */
+    int out_fp32; /* out holds 0: the inputs' type, 1: fp32 (what ring_lse_merge takes) */
+    void* out;
+    int64_t out_token_stride, out_head_stride;
+    float* lse;
+    float softmax_scale;
+    int causal; /* 1: token at place p sees places <= p; 0: all kv_lens[b] places */
+    int window; /* > 0 (causal only): of those, places > p - window, and the first `sinks` */
+    int sinks;
+    /* append: the new rows, [tokens, kv_heads, dim] by strides */
+    const void* k_new;
+    const void* v_new;
+    int64_t k_new_token_stride, k_new_head_stride, v_new_token_stride, v_new_head_stride;
+    /* accumulated attention weight of every place, fp32 [batch, kv_heads, weights_len] by strides, places contiguous */
+    float* weights;
+    int64_t weights_batch_stride, weights_head_stride;
+    int weights_len; /* >= max_pages * page_size */
+    int is_bf16;
+    /* ring_paged_attention_fwd: scratch of at least ring_paged_attention_workspace() bytes, 256-byte aligned */
+    void* workspace;
+    int64_t workspace_bytes;
+    void* stream;
+} Ring_paged_params;
+
+/* Writes the new tokens' K and V rows (k_new, v_new) to their places; a token whose place is negative or in no page is
+ * dropped.  With `weights` the accumulated weight of the new places starts at 0.  Pages that receive rows must not be shared
+ * by two sequences of the call (two rows for one place: either may win).  Asynchronous on `stream`. */
+int ring_paged_append(const Ring_paged_params* params);
+
+/*
+ * Attention of the new tokens over the cache (append first: token i sees its own place):
+ *   out_i = sum_j exp(s_ij - lse_i) v_j,   s_ij = softmax_scale * q_i . k_j,   lse_i = ln sum_j exp(s_ij)
+ * over the places j that token i sees.  A token that sees none gets out = 0, lse = -inf.  Places nobody of a sequence
+ * sees (behind its length, in no page, left of every window) are never read into a result, whatever they hold; a place that
+ * SOME tokens of a sequence see has to hold finite values.  Asynchronous on `stream`; sums and statistics in fp32.
+ */
+int ring_paged_attention_fwd(const Ring_paged_params* params);
+/* Scratch bytes ring_paged_attention_fwd needs for these sizes (pointers of `params` are not looked at), or a negative
+ * RingStatus.  It does not depend on the device contents (lengths, tables). */
+int64_t ring_paged_attention_workspace(const Ring_paged_params* params);
+
+/*
+ * Adds to the weight of every place what the new tokens' attention gave it:
+ *   weights[b, h, j] += sum_i sum_g exp(s_ig,j - lse_ig)     i: tokens of b that see j, g: query heads of K/V head h
+ * with the lse that ring_paged_attention_fwd returned for the same arguments (rows of lse = -inf add nothing).
+ * Every place is added to by one thread in a fixed order: the result does not depend on timing.  Asynchronous on `stream`.
+ */
+int ring_paged_weights(const Ring_paged_params* params);
+
+/*
+ * Eviction by accumulated attention weight.  Of the len places of sequence b, m = min(len, budget) stay, for every K/V head
+ * its own: all if len <= budget; else the first `first`, the last `recent` and, of those between, the budget - first - recent
+ * with the largest weight (ties: the lowest place; NaN counts as the largest).  The kept rows of K and V go, in
+ * their order, to the places 0..m-1 of the pages that dst_table names; those must not hold places of this call's sources (the old pages,
+ * which other sequences may share, stay as they are).  kept[b, h, 0..budget) receives the kept places, ascending, then -1;
+ * new_weights[b, h, 0..new_weights_len) the kept weights, then 0; new_lens[b] = m.  Rows without a page on either side
+ * are not copied.  Asynchronous on `stream`.
+ */
+typedef struct Ring_evict_params {
+    void* k_cache;
+    void* v_cache;
+    int64_t k_page_stride, k_head_stride, k_place_stride;
+    int64_t v_page_stride, v_head_stride, v_place_stride;
+    int num_pages, page_size, kv_heads, dim;
+    const int* page_table;
+    int64_t table_stride;
+    int max_pages;
+    int batch;
+    const int* kv_lens;
+    const int* dst_table;
+    int64_t dst_stride;
+    int dst_pages; /* entries of a dst_table row; dst_pages * page_size >= budget */
+    int budget, first, recent; /* first + recent <= budget */
+    const float* weights;
+    int64_t weights_batch_stride, weights_head_stride;
+    int weights_len; /* >= max_pages * page_size */
+    float* new_weights;
+    int64_t new_weights_batch_stride, new_weights_head_stride;
+    int new_weights_len; /* >= budget */
+    int* kept;     /* [batch, kv_heads, budget] contiguous */
+    int* new_lens; /* [batch] */
+    void* stream;
+} Ring_evict_params;
+int ring_paged_evict(const Ring_evict_params* params);
+
 /* Device status word of the current device: 0, or the code of the bounded wait that ran out
  * (1xx, see csrc/block_attention.cuh).  ring_device_status synchronises the device. */
 int ring_device_status(int* status_out);

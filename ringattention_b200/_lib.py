@@ -51,6 +51,41 @@ class RingStepPlan(ctypes.Structure):
                                      "do_recv", "do_send")]
 
 
+class Ring_paged_params(ctypes.Structure):
+    """Arguments of the paged-cache append, attention and weights calls (include/ring_attention_b200.h)."""
+    _fields_ = [
+        ("k_cache", c_void_p), ("v_cache", c_void_p),
+        ("k_page_stride", c_int64), ("k_head_stride", c_int64), ("k_place_stride", c_int64),
+        ("v_page_stride", c_int64), ("v_head_stride", c_int64), ("v_place_stride", c_int64),
+        ("num_pages", c_int), ("page_size", c_int), ("kv_heads", c_int), ("dim", c_int),
+        ("page_table", c_void_p), ("table_stride", c_int64), ("max_pages", c_int), ("batch", c_int),
+        ("kv_lens", c_void_p), ("cu_seqlens", c_void_p), ("tokens", c_int), ("max_new", c_int),
+        ("q", c_void_p), ("q_token_stride", c_int64), ("q_head_stride", c_int64), ("heads", c_int), ("out_fp32", c_int),
+        ("out", c_void_p), ("out_token_stride", c_int64), ("out_head_stride", c_int64), ("lse", c_void_p),
+        ("softmax_scale", c_float), ("causal", c_int), ("window", c_int), ("sinks", c_int),
+        ("k_new", c_void_p), ("v_new", c_void_p),
+        ("k_new_token_stride", c_int64), ("k_new_head_stride", c_int64), ("v_new_token_stride", c_int64), ("v_new_head_stride", c_int64),
+        ("weights", c_void_p), ("weights_batch_stride", c_int64), ("weights_head_stride", c_int64), ("weights_len", c_int),
+        ("is_bf16", c_int), ("workspace", c_void_p), ("workspace_bytes", c_int64), ("stream", c_void_p),
+    ]
+
+
+class Ring_evict_params(ctypes.Structure):
+    """Arguments of the paged-cache eviction (include/ring_attention_b200.h)."""
+    _fields_ = [
+        ("k_cache", c_void_p), ("v_cache", c_void_p),
+        ("k_page_stride", c_int64), ("k_head_stride", c_int64), ("k_place_stride", c_int64),
+        ("v_page_stride", c_int64), ("v_head_stride", c_int64), ("v_place_stride", c_int64),
+        ("num_pages", c_int), ("page_size", c_int), ("kv_heads", c_int), ("dim", c_int),
+        ("page_table", c_void_p), ("table_stride", c_int64), ("max_pages", c_int), ("batch", c_int), ("kv_lens", c_void_p),
+        ("dst_table", c_void_p), ("dst_stride", c_int64), ("dst_pages", c_int),
+        ("budget", c_int), ("first", c_int), ("recent", c_int),
+        ("weights", c_void_p), ("weights_batch_stride", c_int64), ("weights_head_stride", c_int64), ("weights_len", c_int),
+        ("new_weights", c_void_p), ("new_weights_batch_stride", c_int64), ("new_weights_head_stride", c_int64),
+        ("new_weights_len", c_int), ("kept", c_void_p), ("new_lens", c_void_p), ("stream", c_void_p),
+    ]
+
+
 # name -> (restype, argtypes); every symbol declared in include/ring_attention_b200.h
 SYMBOLS = {
     "ring_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, ctypes.POINTER(c_int), c_int, c_int]),
@@ -77,6 +112,11 @@ SYMBOLS = {
     "ring_lse_merge": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p]),
     "ring_attention_chunked_fwd_static": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                                   c_float, c_int, c_int, c_int, c_void_p]),
+    "ring_paged_append": (c_int, [ctypes.POINTER(Ring_paged_params)]),
+    "ring_paged_attention_fwd": (c_int, [ctypes.POINTER(Ring_paged_params)]),
+    "ring_paged_attention_workspace": (c_int64, [ctypes.POINTER(Ring_paged_params)]),
+    "ring_paged_weights": (c_int, [ctypes.POINTER(Ring_paged_params)]),
+    "ring_paged_evict": (c_int, [ctypes.POINTER(Ring_evict_params)]),
     "ring_device_status": (c_int, [ctypes.POINTER(c_int)]),
     "ring_device_status_reset": (c_int, []),
     "ring_device_status_inject": (c_int, [c_int]),

@@ -23,6 +23,7 @@ __all__ = [
     "ring_attention", "ring_attention_scaled", "set_params_fprop", "Ring_fwd_params", "RingContext",
     "attention_block_fwd", "lse_merge", "device_status", "device_status_reset", "kernel_launch_count",
     "attention_chunked_fwd_static", "static_status",
+    "paged_append", "paged_attention_fwd", "paged_attention_workspace", "paged_weights", "paged_evict",
 ]
 
 
@@ -323,3 +324,211 @@ def static_status(stream=None) -> int:
     s = ctypes.c_int(0)
     check(_lib.load().ring_static_status(ctypes.byref(s), _stream_handle(stream)), "ring_static_status")
     return s.value
+
+
+# ---- paged K/V cache ------------------------------------------------------------------------------------------------
+# The conventions (pages, places, lengths, masks) are those of the C ABI, include/ring_attention_b200.h.  Tensors may have any
+# strides there that are multiples of 8 elements with the last dimension contiguous.  Every call runs on the device of its
+# tensors, on `stream` (default: torch's current stream of that device), and returns without waiting.
+
+def _strided(x, what: str, ndim: int, dtypes, device=None):
+    """(address, strides) of a CUDA tensor whose last dimension is contiguous; strides of one-element dimensions count as 0."""
+    if not hasattr(x, "data_ptr"):
+        raise TypeError(f"{what}: expected a CUDA tensor")
+    if not x.is_cuda:
+        raise ValueError(f"{what} must be a CUDA tensor")
+    if x.dim() != ndim:
+        raise ValueError(f"{what} must have {ndim} dimensions, got {x.dim()}")
+    if x.dtype not in dtypes:
+        raise ValueError(f"{what} has dtype {x.dtype}, expected one of {tuple(dtypes)}")
+    if device is not None and x.device != device:
+        raise ValueError(f"{what} is on {x.device}, expected {device}")
+    if x.shape[-1] > 1 and x.stride(-1) != 1:
+        raise ValueError(f"the last dimension of {what} must be contiguous")
+    return x.data_ptr(), [0 if n == 1 else s for n, s in zip(x.shape[:-1], x.stride()[:-1])]
+
+
+def _distinct(x, what: str) -> None:
+    if any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
+        raise ValueError(f"{what} is written to and must not be an expanded tensor")
+
+
+def _fill_cache(p, k_cache, v_cache, page_table, kv_lens) -> None:
+    import torch
+    half, dev = _half_types(), k_cache.device
+    p.k_cache, (p.k_page_stride, p.k_head_stride, p.k_place_stride) = _strided(k_cache, "k_cache", 4, half)
+    p.num_pages, p.kv_heads, p.page_size, p.dim = k_cache.shape
+    if v_cache is not None:
+        p.v_cache, (p.v_page_stride, p.v_head_stride, p.v_place_stride) = _strided(v_cache, "v_cache", 4, (k_cache.dtype,), dev)
+        if v_cache.shape != k_cache.shape:
+            raise ValueError("k_cache and v_cache must both be [pages, kv_heads, page_size, dim]")
+    p.page_table, (p.table_stride,) = _strided(page_table, "page_table", 2, (torch.int32,), dev)
+    p.batch, p.max_pages = page_table.shape
+    p.kv_lens, _ = _strided(kv_lens, "kv_lens", 1, (torch.int32,), dev)
+    if kv_lens.shape[0] != p.batch:
+        raise ValueError("kv_lens must have one entry per row of page_table")
+
+
+def _fill_tokens(p, tokens: int, cu_seqlens, max_new: int, device) -> None:
+    import torch
+    p.tokens, p.max_new = int(tokens), int(max_new)
+    if cu_seqlens is not None:
+        p.cu_seqlens, _ = _strided(cu_seqlens, "cu_seqlens", 1, (torch.int32,), device)
+        if cu_seqlens.shape[0] != p.batch + 1:
+            raise ValueError("cu_seqlens must have batch + 1 entries")
+
+
+def _fill_queries(p, q, k_cache, lse, softmax_scale, causal, window, sinks) -> None:
+    import torch
+    p.q, (p.q_token_stride, p.q_head_stride) = _strided(q, "q", 3, (k_cache.dtype,), k_cache.device)
+    p.heads = q.shape[1]
+    if q.shape[2] != p.dim:
+        raise ValueError("q must be [tokens, heads, dim] with the cache's dim")
+    if tuple(lse.shape) != tuple(q.shape[:2]) or not lse.is_contiguous():
+        raise ValueError("lse must be a contiguous [tokens, heads]")
+    p.lse, _ = _strided(lse, "lse", 2, (torch.float32,), k_cache.device)
+    p.softmax_scale = float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(p.dim)
+    p.causal, p.window, p.sinks = int(bool(causal)), int(window), int(sinks)
+    p.is_bf16 = int(q.dtype == torch.bfloat16)
+
+
+def _fill_weights(p, weights, device) -> None:
+    import torch
+    p.weights, (p.weights_batch_stride, p.weights_head_stride) = _strided(weights, "weights", 3, (torch.float32,), device)
+    if tuple(weights.shape[:2]) != (p.batch, p.kv_heads):
+        raise ValueError("weights must be [batch, kv_heads, places]")
+    p.weights_len = weights.shape[2]
+
+
+def _on(device, stream):
+    """(context, handle): the device made current, the stream the call goes to."""
+    import torch
+    ctx = torch.cuda.device(device)
+    if stream is None:
+        return ctx, torch.cuda.current_stream(device).cuda_stream
+    return ctx, _stream_handle(stream)
+
+
+def paged_append(k, v, k_cache, v_cache, page_table, kv_lens, *, cu_seqlens=None, weights=None, stream=None) -> None:
+    """Write the new tokens' rows k, v [tokens, kv_heads, dim] to their places in the pages.
+
+    k_cache, v_cache [pages, kv_heads, page_size, dim]; page_table [batch, max_pages], kv_lens [batch] int32, the lengths
+    WITH the new tokens; cu_seqlens [batch + 1] int32 if the sequences bring different numbers of tokens.  weights (see
+    paged_weights) start at 0 at the new places."""
+    p = _lib.Ring_paged_params()
+    _fill_cache(p, k_cache, v_cache, page_table, kv_lens)
+    dev = k_cache.device
+    p.k_new, (p.k_new_token_stride, p.k_new_head_stride) = _strided(k, "k", 3, (k_cache.dtype,), dev)
+    p.v_new, (p.v_new_token_stride, p.v_new_head_stride) = _strided(v, "v", 3, (k_cache.dtype,), dev)
+    if tuple(k.shape) != (k.shape[0], p.kv_heads, p.dim) or v.shape != k.shape:
+        raise ValueError("k and v must both be [tokens, kv_heads, dim]")
+    for x, n in ((k_cache, "k_cache"), (v_cache, "v_cache"), (weights, "weights")):
+        if x is not None:
+            _distinct(x, n)
+    _fill_tokens(p, k.shape[0], cu_seqlens, 0, dev)
+    if weights is not None:
+        _fill_weights(p, weights, dev)
+    ctx, p.stream = _on(dev, stream)
+    with ctx:
+        check(_lib.load().ring_paged_append(ctypes.byref(p)), "ring_paged_append")
+
+
+def paged_attention_workspace(q, k_cache, page_table, *, cu_seqlens=None, max_new: int = 0) -> int:
+    """Bytes of scratch paged_attention_fwd needs for tensors of these shapes (independent of what they hold)."""
+    p = _lib.Ring_paged_params()
+    p.kv_heads, p.dim, p.heads, p.softmax_scale = k_cache.shape[1], k_cache.shape[3], q.shape[1], 1.0
+    p.batch, p.max_pages = page_table.shape
+    _fill_tokens(p, q.shape[0], cu_seqlens, max_new, k_cache.device)
+    import torch
+    with torch.cuda.device(k_cache.device):
+        n = _lib.load().ring_paged_attention_workspace(ctypes.byref(p))
+    if n < 0:
+        check(int(n), "ring_paged_attention_workspace")
+    return int(n)
+
+
+def paged_attention_fwd(q, k_cache, v_cache, page_table, kv_lens, out, lse, *, cu_seqlens=None, max_new: int = 0,
+                        softmax_scale: Optional[float] = None, causal: bool = True, window: int = 0, sinks: int = 0,
+                        workspace=None, stream=None) -> None:
+    """Attention of the new tokens q [tokens, heads, dim] over the paged cache (append their rows first).
+
+    heads is a multiple of the cache's kv_heads.  A token at place p of its sequence sees the places <= p (causal) or all of
+    kv_lens (causal=False); with window > 0 only those > p - window, and the first `sinks`.  out [tokens, heads, dim] in q's
+    type or fp32 (then lse_merge joins the partials of several caches), lse [tokens, heads] fp32.  max_new: an upper
+    bound on the new tokens of one sequence when cu_seqlens is given (helps to choose the kernel).
+    workspace: a uint8 tensor of paged_attention_workspace() bytes of the caller's, for this call alone while it runs;
+    by default one comes from torch's allocator."""
+    import torch
+    p = _lib.Ring_paged_params()
+    _fill_cache(p, k_cache, v_cache, page_table, kv_lens)
+    dev = k_cache.device
+    _fill_queries(p, q, k_cache, lse, softmax_scale, causal, window, sinks)
+    _fill_tokens(p, q.shape[0], cu_seqlens, max_new, dev)
+    if out.shape != q.shape:
+        raise ValueError("out must have q's shape")
+    p.out, (p.out_token_stride, p.out_head_stride) = _strided(out, "out", 3, (q.dtype, torch.float32), dev)
+    _distinct(out, "out")
+    p.out_fp32 = int(out.dtype == torch.float32)
+    ctx, p.stream = _on(dev, stream)
+    with ctx:
+        lib = _lib.load()
+        if workspace is None:
+            n = lib.ring_paged_attention_workspace(ctypes.byref(p))
+            if n < 0:
+                check(int(n), "ring_paged_attention_fwd")
+            # allocated for the stream the call goes to, so that the allocator orders its next user behind this call
+            with torch.cuda.stream(torch.cuda.ExternalStream(p.stream, dev) if p.stream else torch.cuda.default_stream(dev)):
+                workspace = torch.empty(n, dtype=torch.uint8, device=dev)
+        p.workspace, _ = _strided(workspace, "workspace", 1, (torch.uint8,), dev)
+        p.workspace_bytes = workspace.numel()
+        check(lib.ring_paged_attention_fwd(ctypes.byref(p)), "ring_paged_attention_fwd")
+
+
+def paged_weights(weights, q, k_cache, lse, page_table, kv_lens, *, cu_seqlens=None, max_new: int = 0,
+                  softmax_scale: Optional[float] = None, causal: bool = True, window: int = 0, sinks: int = 0, stream=None) -> None:
+    """weights [batch, kv_heads, places] fp32 += the attention that every cached place received from the new tokens: exp(s - lse)
+    summed over the tokens that see it and the query heads of its K/V head, with the lse of paged_attention_fwd for the same
+    arguments.  places >= max_pages * page_size."""
+    p = _lib.Ring_paged_params()
+    _fill_cache(p, k_cache, None, page_table, kv_lens)
+    _fill_queries(p, q, k_cache, lse, softmax_scale, causal, window, sinks)
+    _fill_tokens(p, q.shape[0], cu_seqlens, max_new, k_cache.device)
+    _fill_weights(p, weights, k_cache.device)
+    _distinct(weights, "weights")
+    ctx, p.stream = _on(k_cache.device, stream)
+    with ctx:
+        check(_lib.load().ring_paged_weights(ctypes.byref(p)), "ring_paged_weights")
+
+
+def paged_evict(k_cache, v_cache, weights, page_table, kv_lens, dst_table, budget: int, new_lens, new_weights, kept, *,
+                first: int = 0, recent: int = 0, stream=None) -> None:
+    """Keep at most `budget` places of every sequence and K/V head -- the first `first`, the last `recent` and the heaviest of the
+    others by weights [batch, kv_heads, places] (ties: the lowest place) -- and copy their rows, in order, to the pages
+    dst_table [batch, pages] int32 names, which must not hold places of the sources.  new_lens [batch] int32,
+    new_weights [batch, kv_heads, >= budget] fp32 (0 behind the kept) and kept [batch, kv_heads, budget] int32 (-1 behind) are
+    written."""
+    import torch
+    p = _lib.Ring_evict_params()
+    _fill_cache(p, k_cache, v_cache, page_table, kv_lens)
+    dev = k_cache.device
+    _fill_weights(p, weights, dev)
+    for x, n in ((k_cache, "k_cache"), (v_cache, "v_cache"), (new_weights, "new_weights")):
+        _distinct(x, n)
+    p.dst_table, (p.dst_stride,) = _strided(dst_table, "dst_table", 2, (torch.int32,), dev)
+    if dst_table.shape[0] != p.batch:
+        raise ValueError("dst_table must have one row per row of page_table")
+    p.dst_pages = dst_table.shape[1]
+    p.budget, p.first, p.recent = int(budget), int(first), int(recent)
+    p.new_weights, (p.new_weights_batch_stride, p.new_weights_head_stride) = _strided(new_weights, "new_weights", 3, (torch.float32,), dev)
+    if tuple(new_weights.shape[:2]) != (p.batch, p.kv_heads):
+        raise ValueError("new_weights must be [batch, kv_heads, places]")
+    p.new_weights_len = new_weights.shape[2]
+    if tuple(kept.shape) != (p.batch, p.kv_heads, p.budget) or not kept.is_contiguous():
+        raise ValueError("kept must be a contiguous [batch, kv_heads, budget]")
+    p.kept, _ = _strided(kept, "kept", 3, (torch.int32,), dev)
+    p.new_lens, _ = _strided(new_lens, "new_lens", 1, (torch.int32,), dev)
+    if new_lens.shape[0] != p.batch:
+        raise ValueError("new_lens must have one entry per sequence")
+    ctx, p.stream = _on(dev, stream)
+    with ctx:
+        check(_lib.load().ring_paged_evict(ctypes.byref(p)), "ring_paged_evict")

@@ -12,14 +12,14 @@ import subprocess
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libringattn_b200.so")
-SOURCES = [os.path.join(CSRC, "ring_attention.cu")]
+SOURCES = [os.path.join(CSRC, "ring_attention.cu"), os.path.join(CSRC, "paged.cu")]
 MAIN = os.path.join(HERE, "ring_attention_main")            # the reference's driver executable, over the library
 MAIN_SOURCE = os.path.join(CSRC, "ring_attention_main.cu")
 TORCH_EXT = os.path.join(HERE, "_torch_ext.so")             # torch.Tensor front end (optional; needs torch's headers)
 TORCH_EXT_SOURCE = os.path.join(CSRC, "torch_ext.cpp")
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-    "-shared", "-Xcompiler", "-fPIC",
+    "-shared", "-Xcompiler", "-fPIC", "-t", "0",
 ]
 
 

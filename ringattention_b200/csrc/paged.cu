@@ -1,0 +1,371 @@
+// Host side of the paged-cache operators: argument checks, kernel choice, launches (see ring_attention_b200.h).
+//
+// Nothing here allocates (beyond the library's one-time per-device set-up), waits for the GPU or keeps state between calls.
+#include <cmath>
+#include <cstdint>
+#include <mutex>
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "../../include/ring_attention_b200.h"
+#include "host_common.h"
+#include "paged_cache.cuh"
+#include "paged_plan.cuh"
+#include "paged_rows.cuh"
+
+using namespace ring_host;
+
+namespace {
+
+constexpr int64_t kMaxInt = 0x7fffffff;
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+#define PAGED_REQUIRE(cond, ...) \
+    do {                         \
+        if (!(cond)) return fail(RING_ERR_INVALID_ARGUMENT, __VA_ARGS__); \
+    } while (0)
+
+template <class P>
+int check_cache(const P& p) {
+    PAGED_REQUIRE(p.dim == 64 || p.dim == 128, "dim must be 64 or 128, got %d", p.dim);
+    PAGED_REQUIRE(p.page_size >= 8 && (p.page_size & (p.page_size - 1)) == 0, "page_size must be a power of two >= 8, got %d", p.page_size);
+    PAGED_REQUIRE(p.num_pages >= 1 && p.kv_heads >= 1, "num_pages and kv_heads must be positive");
+    PAGED_REQUIRE(p.max_pages >= 1 && static_cast<int64_t>(p.max_pages) * p.page_size <= (int64_t(1) << 30),
+                  "max_pages must be positive and max_pages * page_size at most 2^30");
+    PAGED_REQUIRE(p.batch >= 1 && p.batch <= 65535, "batch must be in [1, 65535], got %d", p.batch);
+    PAGED_REQUIRE(static_cast<int64_t>(p.batch) * p.kv_heads <= 65535, "batch * kv_heads must not exceed 65535");
+    PAGED_REQUIRE(p.page_table && p.kv_lens, "null page_table or kv_lens");
+    PAGED_REQUIRE(p.table_stride >= p.max_pages || p.batch == 1, "table_stride is smaller than max_pages");
+    PAGED_REQUIRE(p.k_cache, "null k_cache");
+    PAGED_REQUIRE(aligned16(p.k_cache) && aligned16(p.v_cache), "cache base pointers must be 16-byte aligned");
+    const int64_t st = p.k_page_stride | p.k_head_stride | p.k_place_stride | p.v_page_stride | p.v_head_stride | p.v_place_stride;
+    PAGED_REQUIRE((st & 7) == 0, "cache strides must be multiples of 8 elements");
+    PAGED_REQUIRE(p.k_page_stride >= 0 && p.k_head_stride >= 0 && p.k_place_stride >= 0 && p.v_page_stride >= 0 &&
+                      p.v_head_stride >= 0 && p.v_place_stride >= 0, "cache strides must not be negative");
+    return RING_OK;
+}
+
+// A cache that rows are written to: two of its rows must not be one memory (an expanded tensor).
+template <class P>
+int check_written_cache(const P& p) {
+    PAGED_REQUIRE((p.num_pages == 1 || (p.k_page_stride && p.v_page_stride)) && (p.kv_heads == 1 || (p.k_head_stride && p.v_head_stride)) &&
+                      p.k_place_stride && p.v_place_stride, "a cache that is written to must not have strides of 0");
+    return RING_OK;
+}
+
+template <class P>
+void cache_args(const P& p, ring::PagedArgs* a) {
+    *a = ring::PagedArgs{};
+    a->k = p.k_cache;
+    a->v = p.v_cache;
+    a->k_page = p.k_page_stride;
+    a->k_head = p.k_head_stride;
+    a->k_place = p.k_place_stride;
+    a->v_page = p.v_page_stride;
+    a->v_head = p.v_head_stride;
+    a->v_place = p.v_place_stride;
+    a->num_pages = p.num_pages;
+    a->page_shift = __builtin_ctz(static_cast<unsigned>(p.page_size));
+    a->kv_heads = p.kv_heads;
+    a->table = p.page_table;
+    a->table_stride = p.table_stride;
+    a->max_pages = p.max_pages;
+    a->capacity = p.max_pages * p.page_size;
+    a->batch = p.batch;
+    a->lens = p.kv_lens;
+}
+
+int check_tokens(const Ring_paged_params& p) {
+    PAGED_REQUIRE(p.tokens >= 0 && p.max_new >= 0, "tokens and max_new must not be negative");
+    PAGED_REQUIRE(p.cu_seqlens || p.tokens % p.batch == 0, "without cu_seqlens tokens must be a multiple of batch (%d of %d)", p.tokens, p.batch);
+    return RING_OK;
+}
+
+int check_weights(const Ring_paged_params& p) {
+    PAGED_REQUIRE(p.weights_len >= static_cast<int64_t>(p.max_pages) * p.page_size, "weights_len must be at least max_pages * page_size");
+    PAGED_REQUIRE(p.weights_batch_stride >= 0 && p.weights_head_stride >= 0, "weights strides must not be negative");
+    return RING_OK;
+}
+
+// Sizes of a query operand; `pointers` = false leaves the addresses out (the workspace question).
+int check_queries(const Ring_paged_params& p, bool pointers) {
+    int rc = check_tokens(p);
+    if (rc) return rc;
+    PAGED_REQUIRE(p.heads >= 1 && p.heads % p.kv_heads == 0, "heads (%d) must be a positive multiple of kv_heads (%d)", p.heads, p.kv_heads);
+    PAGED_REQUIRE(static_cast<int64_t>(p.tokens) * p.heads <= kMaxInt - 1024, "tokens * heads must stay below 2^31");
+    PAGED_REQUIRE(p.softmax_scale > 0.f && std::isfinite(p.softmax_scale), "softmax_scale must be positive and finite");
+    PAGED_REQUIRE(p.window >= 0 && p.sinks >= 0, "window and sinks must not be negative");
+    PAGED_REQUIRE(p.causal || p.window == 0, "a window needs causal = 1");
+    if (pointers && p.tokens > 0) {
+        PAGED_REQUIRE(p.q && p.lse, "null q or lse");
+        PAGED_REQUIRE(aligned16(p.q), "q must be 16-byte aligned");
+        PAGED_REQUIRE(((p.q_token_stride | p.q_head_stride) & 7) == 0 && p.q_token_stride >= 0 && p.q_head_stride >= 0,
+                      "q strides must be non-negative multiples of 8 elements");
+    }
+    return RING_OK;
+}
+
+void query_args(const Ring_paged_params& p, ring::PagedArgs* a) {
+    cache_args(p, a);
+    a->cu = p.cu_seqlens;
+    a->uniform_new = p.cu_seqlens ? 0 : p.tokens / p.batch;
+    a->tokens = p.tokens;
+    a->q = p.q;
+    a->q_token = p.q_token_stride;
+    a->q_head = p.q_head_stride;
+    a->heads = p.heads;
+    a->group = p.kv_heads ? p.heads / p.kv_heads : 0;
+    a->out_fp32 = p.out_fp32;
+    a->out = p.out;
+    a->out_token = p.out_token_stride;
+    a->out_head = p.out_head_stride;
+    a->lse = p.lse;
+    a->scale = p.softmax_scale;
+    a->scale_log2 = p.softmax_scale * 1.4426950408889634f;
+    a->causal = p.causal ? 1 : 0;
+    a->window = p.window < (1 << 30) ? p.window : 1 << 30;  // no sequence is longer: the same mask, and no sum overflows
+    a->sinks = p.sinks;
+    a->weights = p.weights;
+    a->w_batch = p.weights_batch_stride;
+    a->w_head = p.weights_head_stride;
+}
+
+int max_new_of(const Ring_paged_params& p) {
+    if (!p.cu_seqlens) return p.tokens / p.batch;
+    return p.max_new > 0 && p.max_new < p.tokens ? p.max_new : p.tokens;
+}
+
+template <class Kernel>
+int set_smem(Kernel kernel, int bytes, bool* done) {
+    std::lock_guard<std::mutex> lock(g_dev_mutex);
+    if (!*done) {
+        RING_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        *done = true;
+    }
+    return RING_OK;
+}
+
+// A launch that may begin while the kernel before it in the stream is still running (it waits for that kernel itself).
+template <class... Params, class... Args>
+int launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.stream = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    RING_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return RING_OK;
+}
+
+// ---- attention -----------------------------------------------------------------------------------------------------
+struct AttentionPlan {
+    int unit_rows;
+    int grid;
+    int64_t o_bytes, lse_bytes, cut_bytes;
+    int64_t bytes() const { return o_bytes + lse_bytes + cut_bytes; }
+};
+
+int64_t round256(int64_t x) { return (x + 255) / 256 * 256; }
+
+AttentionPlan attention_plan(const Ring_paged_params& p, int sm_count) {
+    AttentionPlan r;
+    const int64_t rows = static_cast<int64_t>(max_new_of(p)) * (p.heads / p.kv_heads);
+    r.unit_rows = rows <= 16 ? 16 : 32;
+    r.grid = 2 * sm_count;
+    r.o_bytes = round256(int64_t(2) * r.grid * r.unit_rows * p.dim * 4);
+    r.lse_bytes = round256(int64_t(2) * r.grid * r.unit_rows * 4);
+    r.cut_bytes = round256(int64_t(r.grid) * 32);
+    return r;
+}
+
+template <int D, bool kBf16, int MT>
+int launch_rows(const ring::PagedArgs& a, const AttentionPlan& plan, DeviceState* st, cudaStream_t stream) {
+    using T = ring::PagedRowsTraits<D, kBf16, MT>;
+    auto kernel = &ring::ring_paged_rows_kernel<T>;
+    int rc = set_smem(kernel, T::kSmem, &st->paged_attr_set[(MT - 1) * 4 + (D == 128) * 2 + kBf16]);
+    if (rc) return rc;
+    kernel<<<plan.grid, T::kThreads, T::kSmem, stream>>>(a);
+    RING_CUDA(cudaGetLastError());
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return launch_dependent(&ring::ring_paged_join_kernel<D, kBf16, 4>, dim3(plan.grid, 16), dim3(128), stream, a, plan.unit_rows);
+}
+
+template <int D, bool kBf16>
+int launch_attention(const ring::PagedArgs& a, const AttentionPlan& plan, DeviceState* st, cudaStream_t stream) {
+    if (plan.unit_rows == 16) return launch_rows<D, kBf16, 1>(a, plan, st, stream);
+    return launch_rows<D, kBf16, 2>(a, plan, st, stream);
+}
+
+template <int D, bool kBf16>
+int launch_weights(const ring::PagedArgs& a, DeviceState* st, cudaStream_t stream) {
+    using T = ring::PagedWeightsTraits<D, kBf16>;
+    auto kernel = &ring::ring_paged_weights_kernel<T>;
+    int rc = set_smem(kernel, T::kSmem, &st->paged_attr_set[16 + (D == 128) * 2 + kBf16]);
+    if (rc) return rc;
+    kernel<<<dim3((a.capacity + T::kPlaces - 1) / T::kPlaces, a.kv_heads, a.batch), T::kThreads, T::kSmem, stream>>>(a);
+    RING_CUDA(cudaGetLastError());
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return RING_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ring_paged_append(const Ring_paged_params* params) {
+    if (!params) return fail(RING_ERR_INVALID_ARGUMENT, "null params");
+    const Ring_paged_params& p = *params;
+    int rc;
+    if ((rc = check_cache(p)) || (rc = check_written_cache(p)) || (rc = check_tokens(p))) return rc;
+    if (p.weights && (rc = check_weights(p))) return rc;
+    if (p.tokens == 0) return RING_OK;
+    PAGED_REQUIRE(p.v_cache, "null v_cache");
+    PAGED_REQUIRE(p.k_new && p.v_new, "null k_new or v_new");
+    PAGED_REQUIRE(aligned16(p.k_new) && aligned16(p.v_new), "k_new and v_new must be 16-byte aligned");
+    PAGED_REQUIRE(((p.k_new_token_stride | p.k_new_head_stride | p.v_new_token_stride | p.v_new_head_stride) & 7) == 0 &&
+                      p.k_new_token_stride >= 0 && p.k_new_head_stride >= 0 && p.v_new_token_stride >= 0 && p.v_new_head_stride >= 0,
+                  "k_new and v_new strides must be non-negative multiples of 8 elements");
+    ring::PagedAppendArgs args;
+    cache_args(p, &args.a);
+    args.a.cu = p.cu_seqlens;
+    args.a.uniform_new = p.cu_seqlens ? 0 : p.tokens / p.batch;
+    args.a.tokens = p.tokens;
+    args.a.weights = p.weights;
+    args.a.w_batch = p.weights_batch_stride;
+    args.a.w_head = p.weights_head_stride;
+    args.k_new = p.k_new;
+    args.v_new = p.v_new;
+    args.k_token = p.k_new_token_stride;
+    args.k_head = p.k_new_head_stride;
+    args.v_token = p.v_new_token_stride;
+    args.v_head = p.v_new_head_stride;
+    // one pass of the unrolled loop covers 4 * (256 / dim) heads: a warp per pass while there are few tokens
+    const int per_pass = 4 * 256 / p.dim;
+    args.head_parts = (p.kv_heads + per_pass - 1) / per_pass;
+    const int64_t warps = static_cast<int64_t>(p.tokens) * args.head_parts;
+    PAGED_REQUIRE((warps + 7) / 8 <= kMaxInt, "too many tokens");
+    const int blocks = static_cast<int>((warps + 7) / 8);
+    cudaStream_t stream = static_cast<cudaStream_t>(p.stream);
+    if (p.dim == 128)
+        ring::ring_paged_append_kernel<128><<<blocks, 256, 0, stream>>>(args);
+    else
+        ring::ring_paged_append_kernel<64><<<blocks, 256, 0, stream>>>(args);
+    RING_CUDA(cudaGetLastError());
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return RING_OK;
+}
+
+int64_t ring_paged_attention_workspace(const Ring_paged_params* params) {
+    if (!params) return fail(RING_ERR_INVALID_ARGUMENT, "null params");
+    const Ring_paged_params& p = *params;
+    PAGED_REQUIRE(p.dim == 64 || p.dim == 128, "dim must be 64 or 128, got %d", p.dim);
+    PAGED_REQUIRE(p.batch >= 1 && p.kv_heads >= 1, "batch and kv_heads must be positive");
+    int rc = check_queries(p, false);
+    if (rc) return rc;
+    DeviceState* st = nullptr;
+    if ((rc = device_state(&st))) return rc;
+    return attention_plan(p, st->sm_count).bytes();
+}
+
+int ring_paged_attention_fwd(const Ring_paged_params* params) {
+    if (!params) return fail(RING_ERR_INVALID_ARGUMENT, "null params");
+    const Ring_paged_params& p = *params;
+    int rc;
+    if ((rc = check_cache(p)) || (rc = check_queries(p, true))) return rc;
+    if (p.tokens == 0) return RING_OK;
+    PAGED_REQUIRE(p.v_cache && p.out, "null v_cache or out");
+    PAGED_REQUIRE(aligned16(p.out), "out must be 16-byte aligned");
+    const int out_unit = p.out_fp32 ? 3 : 7;
+    PAGED_REQUIRE(((p.out_token_stride | p.out_head_stride) & out_unit) == 0 && p.out_token_stride >= 0 && p.out_head_stride >= 0,
+                  "out strides must be non-negative multiples of 16 bytes");
+    DeviceState* st = nullptr;
+    if ((rc = device_state(&st))) return rc;
+    const AttentionPlan plan = attention_plan(p, st->sm_count);
+    PAGED_REQUIRE(p.workspace && (reinterpret_cast<uintptr_t>(p.workspace) & 255) == 0, "workspace must be 256-byte aligned and not null");
+    PAGED_REQUIRE(p.workspace_bytes >= plan.bytes(), "workspace holds %lld bytes, %lld are needed", (long long)p.workspace_bytes,
+                  (long long)plan.bytes());
+    ring::PagedArgs a;
+    query_args(p, &a);
+    char* ws = static_cast<char*>(p.workspace);
+    a.part_o = reinterpret_cast<float*>(ws);
+    a.part_lse = reinterpret_cast<float*>(ws + plan.o_bytes);
+    a.cut = reinterpret_cast<int4*>(ws + plan.o_bytes + plan.lse_bytes);
+    a.unit_rows = plan.unit_rows;
+    a.many_tiles = (static_cast<int64_t>(max_new_of(p)) * a.group + plan.unit_rows - 1) / plan.unit_rows > 4;
+    a.min_blocks = 1;
+    cudaStream_t stream = static_cast<cudaStream_t>(p.stream);
+    if (p.dim == 128)
+        return p.is_bf16 ? launch_attention<128, true>(a, plan, st, stream) : launch_attention<128, false>(a, plan, st, stream);
+    return p.is_bf16 ? launch_attention<64, true>(a, plan, st, stream) : launch_attention<64, false>(a, plan, st, stream);
+}
+
+int ring_paged_weights(const Ring_paged_params* params) {
+    if (!params) return fail(RING_ERR_INVALID_ARGUMENT, "null params");
+    const Ring_paged_params& p = *params;
+    int rc;
+    if ((rc = check_cache(p)) || (rc = check_queries(p, true)) || (rc = check_weights(p))) return rc;
+    if (p.tokens == 0) return RING_OK;
+    PAGED_REQUIRE(p.weights, "null weights");
+    DeviceState* st = nullptr;
+    if ((rc = device_state(&st))) return rc;
+    ring::PagedArgs a;
+    query_args(p, &a);
+    cudaStream_t stream = static_cast<cudaStream_t>(p.stream);
+    if (p.dim == 128) return p.is_bf16 ? launch_weights<128, true>(a, st, stream) : launch_weights<128, false>(a, st, stream);
+    return p.is_bf16 ? launch_weights<64, true>(a, st, stream) : launch_weights<64, false>(a, st, stream);
+}
+
+int ring_paged_evict(const Ring_evict_params* params) {
+    if (!params) return fail(RING_ERR_INVALID_ARGUMENT, "null params");
+    const Ring_evict_params& p = *params;
+    int rc;
+    if ((rc = check_cache(p)) || (rc = check_written_cache(p))) return rc;
+    PAGED_REQUIRE(p.v_cache, "null v_cache");
+    PAGED_REQUIRE(p.budget >= 1 && p.first >= 0 && p.recent >= 0 && static_cast<int64_t>(p.first) + p.recent <= p.budget,
+                  "budget must be positive and first + recent at most budget (budget %d, first %d, recent %d)", p.budget, p.first, p.recent);
+    PAGED_REQUIRE(p.dst_table && p.dst_pages >= 1 && static_cast<int64_t>(p.dst_pages) * p.page_size >= p.budget,
+                  "dst_table must name pages for %d places", p.budget);
+    PAGED_REQUIRE(p.dst_stride >= p.dst_pages || p.batch == 1, "dst_stride is smaller than dst_pages");
+    PAGED_REQUIRE(p.dst_table != p.page_table, "dst_table must name pages of its own, not the source's");
+    PAGED_REQUIRE(p.weights && p.new_weights && p.kept && p.new_lens, "null weights, new_weights, kept or new_lens");
+    PAGED_REQUIRE(p.weights != p.new_weights, "new_weights must not be weights");
+    PAGED_REQUIRE(p.new_lens != p.kv_lens, "new_lens must not be kv_lens");
+    PAGED_REQUIRE(p.weights_len >= static_cast<int64_t>(p.max_pages) * p.page_size, "weights_len must be at least max_pages * page_size");
+    PAGED_REQUIRE(p.new_weights_len >= p.budget, "new_weights_len must be at least budget");
+    PAGED_REQUIRE(p.weights_batch_stride >= 0 && p.weights_head_stride >= 0 && p.new_weights_batch_stride >= 0 &&
+                      p.new_weights_head_stride >= 0, "weights strides must not be negative");
+    ring::PagedEvictArgs e;
+    cache_args(p, &e.a);
+    e.a.weights = const_cast<float*>(p.weights);
+    e.a.w_batch = p.weights_batch_stride;
+    e.a.w_head = p.weights_head_stride;
+    e.dst_table = p.dst_table;
+    e.dst_stride = p.dst_stride;
+    e.dst_pages = p.dst_pages;
+    e.budget = p.budget;
+    e.first = p.first;
+    e.recent = p.recent;
+    e.new_weights = p.new_weights;
+    e.nw_batch = p.new_weights_batch_stride;
+    e.nw_head = p.new_weights_head_stride;
+    e.nw_len = p.new_weights_len;
+    e.kept = p.kept;
+    e.new_lens = p.new_lens;
+    cudaStream_t stream = static_cast<cudaStream_t>(p.stream);
+    ring::ring_paged_select_kernel<<<p.batch * p.kv_heads, ring::kSelectThreads, 0, stream>>>(e);
+    RING_CUDA(cudaGetLastError());
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    const int per_block = 8 * 4 * (p.dim == 128 ? 1 : 2);
+    const dim3 grid((p.budget + per_block - 1) / per_block, p.batch * p.kv_heads);
+    if (p.dim == 128) return launch_dependent(&ring::ring_paged_gather_kernel<128>, grid, dim3(256), stream, e);
+    return launch_dependent(&ring::ring_paged_gather_kernel<64>, grid, dim3(256), stream, e);
+}
+
+}  // extern "C"

@@ -32,14 +32,15 @@
 #include "../../include/ring_attention_b200.h"
 #include "block_attention.cuh"
 #include "block_attention_pair.cuh"
+#include "host_common.h"
 #include "kernel_traits.h"
 #include "lse_merge.cuh"
 #include "ring.h"
 
-namespace {
+namespace ring_host {
 
 // ------------------------------------------------------------------------------------------ errors
-thread_local std::string g_last_error;
+static thread_local std::string g_last_error;
 
 int fail(int code, const char* fmt, ...) {
     char buf[512];
@@ -51,15 +52,16 @@ int fail(int code, const char* fmt, ...) {
     return code;
 }
 
-#define RING_CUDA(call)                                                                              \
-    do {                                                                                             \
-        cudaError_t e_ = (call);                                                                     \
-        if (e_ != cudaSuccess)                                                                       \
-            return fail(RING_ERR_CUDA, "%s failed: %s (%s:%d)", #call, cudaGetErrorString(e_), __FILE__, \
-                        __LINE__);                                                                   \
-    } while (0)
+static const char* last_error() { return g_last_error.c_str(); }
 
 std::atomic<int64_t> g_launches{0};
+
+}  // namespace ring_host
+
+using namespace ring_host;
+
+namespace {
+
 #ifdef RING_TRACE
 long long* g_trace = nullptr;  // debug builds only: device buffer for clock stamps of one CTA
 #endif
@@ -123,15 +125,13 @@ NcclApi& nccl() {
                         __LINE__);                                                                     \
     } while (0)
 
-// ------------------------------------------------------------------------------------------ per-device state
-struct DeviceState {
-    int* d_status = nullptr;  // device status word written by kernels whose bounded waits ran out
-    int sm_count = 0;
-    bool attr_set[12] = {};  // [one-CTA | pair | pair with two threads per row][dim == 128][bf16]: shared-memory attribute set
-};
+}  // namespace
 
+namespace ring_host {
+
+// ------------------------------------------------------------------------------------------ per-device state
 std::mutex g_dev_mutex;
-DeviceState g_dev[64];
+static DeviceState g_dev[64];
 
 int device_state(DeviceState** out) {
     int dev = 0;
@@ -149,10 +149,6 @@ int device_state(DeviceState** out) {
 }
 
 // ------------------------------------------------------------------------------------------ tensor maps
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
 int encode_fn(EncodeTiledFn* out) {
     static EncodeTiledFn fn = nullptr;
     static std::mutex m;
@@ -168,6 +164,10 @@ int encode_fn(EncodeTiledFn* out) {
     *out = fn;
     return RING_OK;
 }
+
+}  // namespace ring_host
+
+namespace {
 
 // [batch, heads, rows, dim] 16-bit tensor -> 4-D map, box = 64 x 128 x 1 x 1 elements, 128-byte swizzle.
 // Out-of-range rows read as zero, which gives tail predication for free (the reference has none and
@@ -974,7 +974,7 @@ int validate_params(RingCtx* c, const Ring_fwd_params* p) {
 // ------------------------------------------------------------------------------------------ C ABI
 extern "C" {
 
-const char* ring_last_error_string(void) { return g_last_error.c_str(); }
+const char* ring_last_error_string(void) { return last_error(); }
 
 int64_t ring_kernel_launch_count(void) { return g_launches.load(std::memory_order_relaxed); }
 

@@ -52,3 +52,43 @@ def ring_forward(ctx, q, k, v, seqlens: Optional[Sequence[int]] = None, softmax_
 def lse_merge_(o_acc, lse_acc, o_part, lse_part) -> None:
     """Merges the partial (o_part, lse_part) into (o_acc, lse_acc) in place (csrc/ring_attention.cu:439-443, 621-633)."""
     _load().lse_merge_(o_acc, lse_acc, o_part, lse_part)
+
+
+# ---- paged K/V cache: conventions as in include/ring_attention_b200.h; asynchronous on the current stream of the tensors' device ----
+
+def paged_append(k, v, k_cache, v_cache, page_table, kv_lens, cu_seqlens=None, weights=None) -> None:
+    """Writes the new tokens' rows k, v [tokens, kv_heads, dim] to their places in k_cache, v_cache [pages, kv_heads, page_size, dim].
+
+    page_table [batch, max_pages] and kv_lens [batch] are int32; kv_lens counts the new tokens already.  cu_seqlens [batch + 1]
+    int32 when the sequences bring different numbers of tokens.  weights [batch, kv_heads, places]: set to 0 at the new places.
+    """
+    _load().paged_append(k, v, k_cache, v_cache, page_table, kv_lens, cu_seqlens, weights)
+
+
+def paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens=None, max_new: int = 0, softmax_scale: Optional[float] = None,
+                    causal: bool = True, window: int = 0, sinks: int = 0, fp32_out: bool = False) -> Tuple:
+    """Attention of the new tokens q [tokens, heads, dim] over the paged cache: returns (out, lse [tokens, heads] fp32).
+
+    A token at place p sees the places <= p (or, causal=False, all of its sequence); with window > 0 only those > p - window,
+    and the first `sinks`.  out has q's type, or fp32 with fp32_out: the partials of several caches then join with
+    lse_merge_.  max_new bounds the new tokens of one sequence when cu_seqlens is given.  softmax_scale None: 1/sqrt(dim).
+    """
+    return tuple(_load().paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens, max_new, softmax_scale, causal,
+                                         window, sinks, fp32_out))
+
+
+def paged_weights_(weights, q, k_cache, lse, page_table, kv_lens, cu_seqlens=None, max_new: int = 0,
+                   softmax_scale: Optional[float] = None, causal: bool = True, window: int = 0, sinks: int = 0) -> None:
+    """weights [batch, kv_heads, places] += the attention every cached place received from the new tokens, given the lse that
+    paged_attention returned for the same arguments."""
+    _load().paged_weights_(weights, q, k_cache, lse, page_table, kv_lens, cu_seqlens, max_new, softmax_scale, causal, window, sinks)
+
+
+def paged_evict(k_cache, v_cache, weights, page_table, kv_lens, dst_table, budget: int, first: int = 0, recent: int = 0) -> Tuple:
+    """Keeps the first `first`, the last `recent` and the heaviest other places of every sequence and K/V head, `budget` in all, and
+    copies their rows to the pages dst_table names (other pages than the sources).
+
+    Returns (new_lens [batch] int32, new_weights [batch, kv_heads, dst places] fp32, kept [batch, kv_heads, budget] int32,
+    ascending, -1 behind the last).
+    """
+    return tuple(_load().paged_evict(k_cache, v_cache, weights, page_table, kv_lens, dst_table, budget, first, recent))
