@@ -4,13 +4,16 @@
 #include <cmath>
 #include <cstdint>
 #include <mutex>
+#include <type_traits>
 
 #include <cuda.h>
 #include <cuda_runtime.h>
 
 #include "../../include/ring_attention_b200.h"
 #include "host_common.h"
+#include "kernel_traits.h"
 #include "paged_cache.cuh"
+#include "paged_chunk.cuh"
 #include "paged_plan.cuh"
 #include "paged_rows.cuh"
 
@@ -44,14 +47,10 @@ int check_cache(const P& p) {
     PAGED_REQUIRE((st & 7) == 0, "cache strides must be multiples of 8 elements");
     PAGED_REQUIRE(p.k_page_stride >= 0 && p.k_head_stride >= 0 && p.k_place_stride >= 0 && p.v_page_stride >= 0 &&
                       p.v_head_stride >= 0 && p.v_place_stride >= 0, "cache strides must not be negative");
-    return RING_OK;
-}
-
-// A cache that rows are written to: two of its rows must not be one memory (an expanded tensor).
-template <class P>
-int check_written_cache(const P& p) {
-    PAGED_REQUIRE((p.num_pages == 1 || (p.k_page_stride && p.v_page_stride)) && (p.kv_heads == 1 || (p.k_head_stride && p.v_head_stride)) &&
-                      p.k_place_stride && p.v_place_stride, "a cache that is written to must not have strides of 0");
+    // rows of an expanded tensor are one memory: written twice by append, and not a tensor map's either
+    PAGED_REQUIRE((p.num_pages == 1 || (p.k_page_stride && (!p.v_cache || p.v_page_stride))) &&
+                      (p.kv_heads == 1 || (p.k_head_stride && (!p.v_cache || p.v_head_stride))) && p.k_place_stride &&
+                      (!p.v_cache || p.v_place_stride), "cache strides of 0 (an expanded tensor) are not supported");
     return RING_OK;
 }
 
@@ -177,8 +176,8 @@ int64_t round256(int64_t x) { return (x + 255) / 256 * 256; }
 AttentionPlan attention_plan(const Ring_paged_params& p, int sm_count) {
     AttentionPlan r;
     const int64_t rows = static_cast<int64_t>(max_new_of(p)) * (p.heads / p.kv_heads);
-    r.unit_rows = rows <= 16 ? 16 : 32;
-    r.grid = 2 * sm_count;
+    r.unit_rows = rows <= 16 ? 16 : (rows <= 32 ? 32 : 256);
+    r.grid = r.unit_rows <= 32 ? 2 * sm_count : sm_count;  // two CTAs of the few-rows kernel fit an SM, one of the other
     r.o_bytes = round256(int64_t(2) * r.grid * r.unit_rows * p.dim * 4);
     r.lse_bytes = round256(int64_t(2) * r.grid * r.unit_rows * 4);
     r.cut_bytes = round256(int64_t(r.grid) * 32);
@@ -197,8 +196,45 @@ int launch_rows(const ring::PagedArgs& a, const AttentionPlan& plan, DeviceState
     return launch_dependent(&ring::ring_paged_join_kernel<D, kBf16, 4>, dim3(plan.grid, 16), dim3(128), stream, a, plan.unit_rows);
 }
 
+// The cache as a 4-D map [pages, kv_heads, page_size, dim]: a box is 64 columns of min(page_size, 128) places of one page and head,
+// 128-byte swizzle.  Page num_pages reads as zeros.
+int cache_map(CUtensorMap* tm, const ring::PagedArgs& a, const void* base, int64_t page, int64_t head, int64_t place, int dim, bool bf16) {
+    EncodeTiledFn enc = nullptr;
+    int rc = encode_fn(&enc);
+    if (rc) return rc;
+    const int page_size = 1 << a.page_shift;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(page_size), static_cast<cuuint64_t>(a.kv_heads),
+                                static_cast<cuuint64_t>(a.num_pages)};
+    // a dimension of one element may come with any stride
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(place) * 2, static_cast<cuuint64_t>(a.kv_heads == 1 ? dim : head) * 2,
+                                   static_cast<cuuint64_t>(a.num_pages == 1 ? dim : page) * 2};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(page_size < 128 ? page_size : 128), 1, 1};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    const CUresult r = enc(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims,
+                           strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(RING_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+    return RING_OK;
+}
+
+template <int D, bool kBf16>
+int launch_chunk(const ring::PagedArgs& a, const AttentionPlan& plan, DeviceState* st, cudaStream_t stream) {
+    using T = Ring_fwd_traits<D, 256, 128, 12, typename std::conditional<kBf16, __nv_bfloat16, __half>::type>;
+    auto kernel = &ring::ring_paged_chunk_kernel<T>;
+    int rc = set_smem(kernel, T::kSmemSize, &st->paged_attr_set[8 + (D == 128) * 2 + kBf16]);
+    if (rc) return rc;
+    CUtensorMap tk, tv;
+    if ((rc = cache_map(&tk, a, a.k, a.k_page, a.k_head, a.k_place, D, kBf16))) return rc;
+    if ((rc = cache_map(&tv, a, a.v, a.v_page, a.v_head, a.v_place, D, kBf16))) return rc;
+    kernel<<<plan.grid, T::kNThreads, T::kSmemSize, stream>>>(tk, tv, a);
+    RING_CUDA(cudaGetLastError());
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return launch_dependent(&ring::ring_paged_join_kernel<D, kBf16, 1>, dim3(plan.grid, 32), dim3(128), stream, a, plan.unit_rows);
+}
+
 template <int D, bool kBf16>
 int launch_attention(const ring::PagedArgs& a, const AttentionPlan& plan, DeviceState* st, cudaStream_t stream) {
+    if (plan.unit_rows == 256) return launch_chunk<D, kBf16>(a, plan, st, stream);
     if (plan.unit_rows == 16) return launch_rows<D, kBf16, 1>(a, plan, st, stream);
     return launch_rows<D, kBf16, 2>(a, plan, st, stream);
 }
@@ -223,7 +259,7 @@ int ring_paged_append(const Ring_paged_params* params) {
     if (!params) return fail(RING_ERR_INVALID_ARGUMENT, "null params");
     const Ring_paged_params& p = *params;
     int rc;
-    if ((rc = check_cache(p)) || (rc = check_written_cache(p)) || (rc = check_tokens(p))) return rc;
+    if ((rc = check_cache(p)) || (rc = check_tokens(p))) return rc;
     if (p.weights && (rc = check_weights(p))) return rc;
     if (p.tokens == 0) return RING_OK;
     PAGED_REQUIRE(p.v_cache, "null v_cache");
@@ -299,7 +335,8 @@ int ring_paged_attention_fwd(const Ring_paged_params* params) {
     a.cut = reinterpret_cast<int4*>(ws + plan.o_bytes + plan.lse_bytes);
     a.unit_rows = plan.unit_rows;
     a.many_tiles = (static_cast<int64_t>(max_new_of(p)) * a.group + plan.unit_rows - 1) / plan.unit_rows > 4;
-    a.min_blocks = 1;
+    a.min_blocks = plan.unit_rows == 256 ? 2 : 1;
+    a.status = plan.unit_rows == 256 ? st->d_status : nullptr;
     cudaStream_t stream = static_cast<cudaStream_t>(p.stream);
     if (p.dim == 128)
         return p.is_bf16 ? launch_attention<128, true>(a, plan, st, stream) : launch_attention<128, false>(a, plan, st, stream);
@@ -326,7 +363,7 @@ int ring_paged_evict(const Ring_evict_params* params) {
     if (!params) return fail(RING_ERR_INVALID_ARGUMENT, "null params");
     const Ring_evict_params& p = *params;
     int rc;
-    if ((rc = check_cache(p)) || (rc = check_written_cache(p))) return rc;
+    if ((rc = check_cache(p))) return rc;
     PAGED_REQUIRE(p.v_cache, "null v_cache");
     PAGED_REQUIRE(p.budget >= 1 && p.first >= 0 && p.recent >= 0 && static_cast<int64_t>(p.first) + p.recent <= p.budget,
                   "budget must be positive and first + recent at most budget (budget %d, first %d, recent %d)", p.budget, p.first, p.recent);

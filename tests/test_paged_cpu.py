@@ -50,7 +50,7 @@ CACHE = [
     (dict(batch=65536), "batch"), (dict(batch=40000, tokens=40000), "65535"), (dict(page_table=None), "page_table"),
     (dict(kv_lens=None), "kv_lens"), (dict(table_stride=3), "table_stride"), (dict(k_cache=None), "k_cache"),
     (dict(k_cache=0x1008), "16-byte aligned"), (dict(k_place_stride=60), "multiples of 8"), (dict(v_head_stride=4), "multiples of 8"),
-    (dict(k_page_stride=-64), "negative"),
+    (dict(k_page_stride=-64), "negative"), (dict(k_head_stride=0), "strides of 0"), (dict(k_place_stride=0), "strides of 0"),
 ]
 
 

@@ -17,6 +17,13 @@ def ops():
     return torch_ops
 
 
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    import ringattention_b200 as ra
+    yield
+    assert ra.device_status() == 0
+
+
 def attend(ops, s, **kw):
     return ops.paged_attention(s.q, s.k_cache, s.v_cache, s.table, s.kv_lens, cu_seqlens=s.cu, max_new=kw.pop("max_new", s.max_new), **kw)
 
