@@ -166,6 +166,7 @@ int launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, cudaStrea
 // ---- attention -----------------------------------------------------------------------------------------------------
 struct AttentionPlan {
     int unit_rows;
+    int rows;  // rows a unit of the few-rows kernel is expected to have
     int grid;
     int64_t o_bytes, lse_bytes, cut_bytes;
     int64_t bytes() const { return o_bytes + lse_bytes + cut_bytes; }
@@ -177,6 +178,7 @@ AttentionPlan attention_plan(const Ring_paged_params& p, int sm_count) {
     AttentionPlan r;
     const int64_t rows = static_cast<int64_t>(max_new_of(p)) * (p.heads / p.kv_heads);
     r.unit_rows = rows <= 16 ? 16 : (rows <= 32 ? 32 : 256);
+    r.rows = static_cast<int>(rows < 1 ? 1 : (rows < r.unit_rows ? rows : r.unit_rows));
     r.grid = r.unit_rows <= 32 ? 2 * sm_count : sm_count;  // two CTAs of the few-rows kernel fit an SM, one of the other
     r.o_bytes = round256(int64_t(2) * r.grid * r.unit_rows * p.dim * 4);
     r.lse_bytes = round256(int64_t(2) * r.grid * r.unit_rows * 4);
@@ -193,7 +195,7 @@ int launch_rows(const ring::PagedArgs& a, const AttentionPlan& plan, DeviceState
     kernel<<<plan.grid, T::kThreads, T::kSmem, stream>>>(a);
     RING_CUDA(cudaGetLastError());
     g_launches.fetch_add(1, std::memory_order_relaxed);
-    return launch_dependent(&ring::ring_paged_join_kernel<D, kBf16, 4>, dim3(plan.grid, 16), dim3(128), stream, a, plan.unit_rows);
+    return launch_dependent(&ring::ring_paged_join_kernel<D, kBf16, 4>, dim3(plan.grid, plan.rows), dim3(128), stream, a, plan.unit_rows);
 }
 
 // The cache as a 4-D map [pages, kv_heads, page_size, dim]: a box is 64 columns of min(page_size, 128) places of one page and head,
@@ -335,7 +337,8 @@ int ring_paged_attention_fwd(const Ring_paged_params* params) {
     a.cut = reinterpret_cast<int4*>(ws + plan.o_bytes + plan.lse_bytes);
     a.unit_rows = plan.unit_rows;
     a.many_tiles = (static_cast<int64_t>(max_new_of(p)) * a.group + plan.unit_rows - 1) / plan.unit_rows > 4;
-    a.min_blocks = plan.unit_rows == 256 ? 2 : 1;
+    a.start_cost = plan.unit_rows == 256 ? 3 : 2;
+    a.min_blocks = a.start_cost + (plan.unit_rows == 256 ? 2 : 1);
     a.status = plan.unit_rows == 256 ? st->d_status : nullptr;
     cudaStream_t stream = static_cast<cudaStream_t>(p.stream);
     if (p.dim == 128)

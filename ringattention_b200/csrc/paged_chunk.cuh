@@ -99,8 +99,10 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     }
     __syncthreads();
     if (*prior_error != 0) return;  // an earlier launch failed: do nothing (CTA-uniform)
-    plan_start<BN, T::kNThreads>(a, plan, cta, gridDim.x);
-    if (!plan.seg.valid) return;  // no share (CTA-uniform)
+    using U = AttentionUnits<BN>;
+    Share share;
+    Segment g = plan_start<U, T::kNThreads>(a, plan, share, cta, gridDim.x);
+    if (!g.valid) return;  // no share (CTA-uniform)
 
     if (warp == T::kMmaWarp) {
         tmem_alloc(smem_u32(tmem_slot), T::kTmemCols);
@@ -112,14 +114,12 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     const uint32_t tmem_base = *tmem_slot;
 
     // ---- what every role knows of the current segment, and how far its barriers have come
-    Segment g = plan.seg;
     SeqView s;
     TileBlocks tb;
     int row0, rows, ntiles, hi_max, lo_min;
     uint32_t kv_done = 0;              // K/V blocks of earlier segments
     uint32_t tile1_done = 0;           // ... of those that had a second tile (the first tile takes part in all)
     uint32_t segs_done = 0, segs1_done = 0;  // segments, and those with a second tile
-    int64_t x = plan.x0;
     auto begin_segment = [&]() {
         s = seq_view(a, g.b);
         row0 = g.tile * a.unit_rows;
@@ -141,10 +141,7 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             tile1_done += g.count;
             ++segs1_done;
         }
-        x += g.count;
-        if (tid == 0) plan.seg = plan_next<BN>(a, g, plan.x1 - x);
-        bar_sync_all(T::kNThreads);
-        g = plan.seg;
+        g = plan_next<U>(a, share, g);
         return g.valid != 0;
     };
 
@@ -508,7 +505,7 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                         else
                             a.lse[static_cast<int64_t>(s.q0 + tok) * a.heads + g.h * a.group + (row0 + row - tok * a.group)] = lse;
                     }
-                    if (slot == 2 * cta + 1 && tid == 0) note_cut(a, plan, g, cta, x, row0, rows, s.q0);
+                    if (slot == 2 * cta + 1 && tid == 0) note_cut(a, share, g, cta, row0, rows, s.q0);
                 }
             }
         } while (end_segment());

@@ -2,10 +2,11 @@
 // of a ragged batch out to CTAs on the device.
 //
 // The lengths of the sequences live on the device and no call waits for them, so the host cannot size a grid by them.  The
-// attention kernels therefore run a fixed grid of resident CTAs; each computes the total number of key blocks that all units
-// (sequence, K/V head, tile of query rows) have to visit, takes its equal share [c T / n, (c + 1) T / n) of that list, and
-// walks the units in it.  A unit that a share boundary cuts leaves normalised partials with their LSE in the
-// workspace, which a second small kernel joins (the algebra of lse_merge.cuh over many partials).  So a batch of one long
+// kernels therefore run a fixed grid of resident CTAs; each computes the total cost of all units (sequence, K/V head, tile: of
+// query rows for attention, of places for the weights), takes its equal share [c T / n, (c + 1) T / n) of that list, and
+// walks the units in it.  A unit costs its blocks plus a constant for starting it: without the constant the CTA that got
+// a batch's short sequences and idle slots finished last (b32 ragged to 8192, 8 K/V heads: busiest SM 1.35 times the mean).  A unit
+// that a share boundary cuts leaves partials in the workspace, which a second small kernel joins.  So a batch of one long
 // sequence and thirty short ones keeps every SM equally busy, and a single sequence is cut as finely as there are CTAs.
 #pragma once
 
@@ -37,7 +38,8 @@ struct PagedArgs {
     int causal, window, sinks;
     int unit_rows;    // query rows (token-major, then head of the group) per unit
     int many_tiles;   // hint: a sequence may have many tiles, sum its blocks with a warp instead of a thread
-    int min_blocks;   // key blocks a CTA should at least get
+    int min_blocks;   // cost a CTA should at least get
+    int start_cost;   // cost of starting a unit, in blocks
     float* weights;
     int64_t w_batch, w_head;
     // workspace of the attention kernels: part_o [2 * grid][unit_rows][D], part_lse [2 * grid][unit_rows], cut [grid]
@@ -111,181 +113,215 @@ __device__ __forceinline__ int tile_rows(const PagedArgs& a, const SeqView& s, i
     return min(a.unit_rows, s.n * a.group - tile * a.unit_rows);
 }
 
+// What the attention kernels deal out: tiles of unit_rows query rows, with the BN-place key blocks each has to visit.
+template <int BN>
+struct AttentionUnits {
+    static __device__ __forceinline__ int tiles(const PagedArgs& a, const SeqView& s) { return seq_tiles(a, s); }
+    static __device__ __forceinline__ int blocks(const PagedArgs& a, const SeqView& s, int tile) {
+        return tile_blocks<BN>(a, s, tile * a.unit_rows, tile_rows(a, s, tile)).count;
+    }
+};
+
 // One unit's piece in a CTA's share.
 struct Segment {
     int b, h, tile;
-    int first, count;  // index of the first of the unit's blocks to visit, and how many
+    int tiles;        // of the sequence
+    int first, count; // index of the first of the unit's blocks to visit, and how many
     int unit_blocks;
-    int tiles;   // of the sequence
     int valid;
+    int64_t begin;    // where the unit begins in the list of costs
 };
 
-struct PlanShared {
-    int64_t warp_sum[33];
-    int64_t total;  // key blocks per K/V head, over all sequences
-    int found_b;
-    int64_t found_before;
-    int64_t found_own;
-    Segment seg;
-    int active;       // CTAs that have a share
-    int64_t x0, x1;   // this CTA's share
+// A CTA's share [x0, x1) of the list of costs.
+struct Share {
+    int64_t all;  // the whole list
+    int active;   // CTAs that have a share
+    int64_t x0, x1;
 };
 
-// Sum of the sequence's tile blocks (one K/V head), by one warp (all lanes call it, all get the sum).
-template <int BN>
-__device__ __forceinline__ int64_t seq_blocks_warp(const PagedArgs& a, const SeqView& s) {
-    const int tiles = seq_tiles(a, s);
+__device__ __forceinline__ int64_t share_begin(int64_t all, int c, int n) {
+    if (all < (1 << 21)) return static_cast<uint32_t>(all) * static_cast<uint32_t>(c) / static_cast<uint32_t>(n);  // c, n < 2^11
+    return all * c / n;
+}
+
+__device__ __forceinline__ Share make_share(const PagedArgs& a, int64_t all, int cta, int ctas) {
+    Share r;
+    r.all = all;
+    const int64_t want = all < (1 << 30) ? static_cast<uint32_t>(all + a.min_blocks - 1) / static_cast<uint32_t>(a.min_blocks) : ctas;
+    r.active = static_cast<int>(want < ctas ? want : ctas);
+    r.x0 = r.x1 = 0;
+    if (cta < r.active) {
+        r.x0 = share_begin(all, cta, r.active);
+        r.x1 = share_begin(all, cta + 1, r.active);
+    }
+    return r;
+}
+
+// Cost of the sequence's units for one K/V head: by one thread, or by a warp (all its lanes call it and get the sum).
+template <class U>
+__device__ __forceinline__ int64_t seq_cost_thread(const PagedArgs& a, const SeqView& s) {
+    const int tiles = U::tiles(a, s);
     int64_t sum = 0;
-    for (int t = threadIdx.x & 31; t < tiles; t += 32)
-        sum += tile_blocks<BN>(a, s, t * a.unit_rows, tile_rows(a, s, t)).count;
+    for (int t = 0; t < tiles; ++t) sum += U::blocks(a, s, t) + a.start_cost;
+    return sum;
+}
+template <class U>
+__device__ __forceinline__ int64_t seq_cost_warp(const PagedArgs& a, const SeqView& s) {
+    const int tiles = U::tiles(a, s);
+    int64_t sum = 0;
+    for (int t = threadIdx.x & 31; t < tiles; t += 32) sum += U::blocks(a, s, t) + a.start_cost;
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     return sum;
 }
-template <int BN>
-__device__ __forceinline__ int64_t seq_blocks_thread(const PagedArgs& a, const SeqView& s) {
-    const int tiles = seq_tiles(a, s);
-    int64_t sum = 0;
-    for (int t = 0; t < tiles; ++t) sum += tile_blocks<BN>(a, s, t * a.unit_rows, tile_rows(a, s, t)).count;
-    return sum;
+
+// The piece of a unit that begins at `g.begin` (g.b, h, tile, tiles, unit_blocks set) inside [from, x1).
+__device__ __forceinline__ void cut_unit(const PagedArgs& a, Segment& g, int64_t from, int64_t x1) {
+    const int64_t blocks0 = g.begin + a.start_cost;
+    g.first = from > blocks0 ? static_cast<int>(from - blocks0) : 0;
+    const int64_t end = x1 - blocks0;
+    g.count = static_cast<int>(end < g.unit_blocks ? end : g.unit_blocks) - g.first;
+    g.valid = g.count > 0;
 }
 
-// Exclusive prefix over the block's threads; *total receives the sum.  Every thread calls it.
-template <int kThreads>
-__device__ __forceinline__ int64_t block_prefix(PlanShared& p, int64_t v, int64_t* total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int64_t x = v;
+// The first segment of the share: x0 lies in sequence b, whose list begins at `before` and costs `own` per head.  Called by a
+// whole warp, which gets the result in every lane.
+template <class U>
+__device__ __forceinline__ Segment first_segment(const PagedArgs& a, const Share& sh, int b, int64_t before, int64_t own) {
+    const int lane = threadIdx.x & 31;
+    const SeqView s = seq_view(a, b);
+    Segment g;
+    g.b = b;
+    const int64_t rel = sh.x0 - before;
+    g.h = rel < (1 << 30) && own < (1 << 30) ? static_cast<int>(static_cast<uint32_t>(rel) / static_cast<uint32_t>(own))
+                                              : static_cast<int>(rel / own);
+    g.tiles = U::tiles(a, s);
+    int64_t at = before + g.h * own;  // list position of the tiles looked at
+    g.tile = 0;
+    g.begin = at;
+    g.unit_blocks = 0;
+    for (int t0 = 0; t0 < g.tiles; t0 += 32) {
+        const int t = t0 + lane;
+        const int c = t < g.tiles ? U::blocks(a, s, t) + a.start_cost : 0;
+        int x = c;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-    }
-    if (lane == 31) p.warp_sum[warp] = x;
-    __syncthreads();
-    int64_t before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) {
-        const int64_t y = p.warp_sum[w];
-        if (w < warp) before += y;
-        all += y;
-    }
-    __syncthreads();
-    *total = all;
-    return before + x - v;
-}
-
-// This thread's sequence of the chunk starting at b0: its blocks per K/V head (0 past the batch).
-// kSlots sequences per chunk: one per thread, or one per warp when sequences may have many tiles.
-template <int BN, int kThreads>
-__device__ __forceinline__ int64_t chunk_blocks(const PagedArgs& a, int b0, int* b_out) {
-    int64_t own = 0;
-    int b;
-    if (a.many_tiles) {
-        b = b0 + (threadIdx.x >> 5);
-        if (b < a.batch) {
-            own = seq_blocks_warp<BN>(a, seq_view(a, b));
-            if (threadIdx.x & 31) own = 0;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
         }
-        if (threadIdx.x & 31) b = -1;
-    } else {
-        b = b0 + threadIdx.x;
-        if (b < a.batch) own = seq_blocks_thread<BN>(a, seq_view(a, b));
+        const unsigned hit = __ballot_sync(0xffffffffu, c > 0 && sh.x0 < at + x);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            g.tile = t0 + l;
+            g.unit_blocks = __shfl_sync(0xffffffffu, c, l) - a.start_cost;
+            g.begin = at + __shfl_sync(0xffffffffu, x - c, l);
+            break;
+        }
+        at += __shfl_sync(0xffffffffu, x, 31);
     }
-    *b_out = b;
-    return own;
+    cut_unit(a, g, sh.x0, sh.x1);
+    return g;
 }
 
-// Computes this CTA's share and its first segment into `p` (all threads call it; ends in a __syncthreads).
-template <int BN, int kThreads>
-__device__ void plan_start(const PagedArgs& a, PlanShared& p, int cta, int ctas) {
+struct PlanShared {
+    int64_t warp_sum[32];
+    int found_b;
+    int64_t found_before, found_own;
+};
+
+// This CTA's share and its first segment (all threads call it and get the same; `p` is scratch).
+template <class U, int kThreads>
+__device__ __forceinline__ Segment plan_start(const PagedArgs& a, PlanShared& p, Share& sh, int cta, int ctas) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    Segment none;
+    none.valid = 0;
+    if (a.batch <= 32) {
+        // every warp works it out for itself: no barrier on the way to the first load
+        int64_t own = 0;
+        if (a.many_tiles) {
+            for (int b = 0; b < a.batch; ++b) {
+                const int64_t c = seq_cost_warp<U>(a, seq_view(a, b));
+                if (lane == b) own = c;
+            }
+        } else if (lane < a.batch) {
+            own = seq_cost_thread<U>(a, seq_view(a, lane));
+        }
+        int64_t x = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        sh = make_share(a, __shfl_sync(0xffffffffu, x, 31) * a.kv_heads, cta, ctas);
+        if (sh.x0 >= sh.x1) return none;
+        const unsigned hit = __ballot_sync(0xffffffffu, own > 0 && sh.x0 < x * a.kv_heads);
+        const int b = __ffs(hit) - 1;
+        return first_segment<U>(a, sh, b, __shfl_sync(0xffffffffu, x - own, b) * a.kv_heads, __shfl_sync(0xffffffffu, own, b));
+    }
+    // larger batches: a sequence per thread (per warp if they may have many tiles), prefix sums over the CTA
     const int step = a.many_tiles ? kThreads / 32 : kThreads;
-    const bool single = a.batch <= step;
-    int64_t total = 0, own = 0, before = 0, chunk_total = 0;
+    int64_t total = 0;
+    auto chunk = [&](int b0, int* b_out, int64_t* own_out, int64_t* chunk_total) {
+        int64_t own = 0;
+        int b;
+        if (a.many_tiles) {
+            b = b0 + warp;
+            if (b < a.batch) own = seq_cost_warp<U>(a, seq_view(a, b));
+            if (lane) own = 0;
+        } else {
+            b = b0 + threadIdx.x;
+            if (b < a.batch) own = seq_cost_thread<U>(a, seq_view(a, b));
+        }
+        int64_t x = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        __syncthreads();
+        if (lane == 31) p.warp_sum[warp] = x;
+        __syncthreads();
+        int64_t before = 0, all = 0;
+#pragma unroll
+        for (int w = 0; w < kThreads / 32; ++w) {
+            const int64_t y = p.warp_sum[w];
+            if (w < warp) before += y;
+            all += y;
+        }
+        *b_out = b;
+        *own_out = own;
+        *chunk_total = all;
+        return before + x - own;
+    };
     int b = 0;
+    int64_t own = 0, chunk_total = 0;
     for (int b0 = 0; b0 < a.batch; b0 += step) {
-        own = chunk_blocks<BN, kThreads>(a, b0, &b);
-        before = block_prefix<kThreads>(p, own, &chunk_total);
+        chunk(b0, &b, &own, &chunk_total);
         total += chunk_total;
     }
-    const int64_t all = total * a.kv_heads;
-    int64_t want = (all + a.min_blocks - 1) / a.min_blocks;
-    const int active = static_cast<int>(want < ctas ? want : ctas);
-    int64_t x0 = 0, x1 = 0;
-    if (cta < active) {
-        x0 = all * cta / active;
-        x1 = all * (cta + 1) / active;
-    }
-    if (threadIdx.x == 0) {
-        p.total = total;
-        p.active = active;
-        p.x0 = x0;
-        p.x1 = x1;
-        p.found_b = -1;
-        p.seg.valid = 0;
-    }
-    __syncthreads();
-    if (x0 >= x1) return;  // CTA-uniform
-    // the sequence whose units hold block x0
+    sh = make_share(a, total * a.kv_heads, cta, ctas);
+    if (sh.x0 >= sh.x1) return none;  // CTA-uniform
     int64_t done = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += step) {
-        if (!single) {
-            own = chunk_blocks<BN, kThreads>(a, b0, &b);
-            before = block_prefix<kThreads>(p, own, &chunk_total);
-        }
-        const int64_t lo = (done + before) * a.kv_heads, hi = lo + own * a.kv_heads;
-        if (own > 0 && x0 >= lo && x0 < hi) {
+    for (int b0 = 0; b0 < a.batch && done * a.kv_heads <= sh.x0; b0 += step) {
+        const int64_t before = chunk(b0, &b, &own, &chunk_total);
+        const int64_t lo = (done + before) * a.kv_heads;
+        if (own > 0 && sh.x0 >= lo && sh.x0 < lo + own * a.kv_heads) {
             p.found_b = b;
             p.found_before = lo;
             p.found_own = own;
         }
         done += chunk_total;
-        if (done * a.kv_heads > x0) break;  // CTA-uniform
     }
     __syncthreads();
-    // the head and the tile within it: one warp
-    if (threadIdx.x < 32) {
-        const int fb = p.found_b;
-        const SeqView s = seq_view(a, fb);
-        const int h = static_cast<int>((x0 - p.found_before) / p.found_own);
-        int64_t rest = (x0 - p.found_before) - h * p.found_own;
-        const int tiles = seq_tiles(a, s);
-        for (int t0 = 0; t0 < tiles; t0 += 32) {
-            const int t = t0 + threadIdx.x;
-            int c = t < tiles ? tile_blocks<BN>(a, s, t * a.unit_rows, tile_rows(a, s, t)).count : 0;
-            int x = c;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, x, o);
-                if (threadIdx.x >= o) x += y;
-            }
-            const int sum = __shfl_sync(0xffffffffu, x, 31);
-            if (rest < sum) {
-                if (c > 0 && rest >= x - c && rest < x) {
-                    Segment g;
-                    g.b = fb;
-                    g.h = h;
-                    g.tile = t;
-                    g.tiles = tiles;
-                    g.unit_blocks = c;
-                    g.first = static_cast<int>(rest) - (x - c);
-                    const int64_t left = x1 - x0;
-                    g.count = static_cast<int>(left < c - g.first ? left : c - g.first);
-                    g.valid = 1;
-                    p.seg = g;
-                }
-                break;
-            }
-            rest -= sum;
-        }
-    }
-    __syncthreads();
+    return first_segment<U>(a, sh, p.found_b, p.found_before, p.found_own);
 }
 
-// The segment after `g` in a share that has `left` blocks remaining behind g.  One thread.
-template <int BN>
-__device__ __forceinline__ Segment plan_next(const PagedArgs& a, Segment g, int64_t left) {
+// The segment after `g` in the share.  Every thread that needs it works it out.
+template <class U>
+__device__ __forceinline__ Segment plan_next(const PagedArgs& a, const Share& sh, Segment g) {
+    const int64_t at = g.begin + a.start_cost + g.unit_blocks;  // where the next unit begins
     g.valid = 0;
-    if (left <= 0) return g;
+    if (g.first + g.count < g.unit_blocks || at >= sh.x1) return g;
     SeqView s;
     if (g.tile + 1 < g.tiles) {
         ++g.tile;
@@ -300,13 +336,12 @@ __device__ __forceinline__ Segment plan_next(const PagedArgs& a, Segment g, int6
         do {
             if (++g.b >= a.batch) return g;
             s = seq_view(a, g.b);
-        } while (s.n == 0);
-        g.tiles = seq_tiles(a, s);
+            g.tiles = U::tiles(a, s);
+        } while (g.tiles == 0);
     }
-    g.unit_blocks = tile_blocks<BN>(a, s, g.tile * a.unit_rows, tile_rows(a, s, g.tile)).count;
-    g.first = 0;
-    g.count = static_cast<int>(left < g.unit_blocks ? left : g.unit_blocks);
-    g.valid = 1;
+    g.begin = at;
+    g.unit_blocks = U::blocks(a, s, g.tile);
+    cut_unit(a, g, at, sh.x1);
     return g;
 }
 
@@ -316,18 +351,20 @@ __device__ __forceinline__ int partial_slot(const Segment& g, int cta) {
     return g.first > 0 ? 2 * cta : 2 * cta + 1;
 }
 
-// CTA `cta` notes the unit that begins in its share and ends behind it (parts = 0: there is none).
-__device__ __forceinline__ void note_cut(const PagedArgs& a, const PlanShared& p, const Segment& g, int cta, int64_t x_seg, int row0,
-                                         int rows, int q0) {
-    // the unit ends at block x_seg - first + unit_blocks; the CTA that holds its last block is the largest c with
-    // all * c / active <= that block
-    const int64_t all = p.total * a.kv_heads;
-    const int64_t last = x_seg - g.first + g.unit_blocks - 1;
-    int64_t c = last * p.active / all;
-    while (c + 1 < p.active && all * (c + 1) / p.active <= last) ++c;
-    while (c > 0 && all * c / p.active > last) --c;
+// The CTA whose share holds list position x.
+__device__ __forceinline__ int cta_of(const Share& sh, int64_t x) {
+    int c = static_cast<int>(x * sh.active / sh.all);
+    while (c + 1 < sh.active && share_begin(sh.all, c + 1, sh.active) <= x) ++c;
+    while (c > 0 && share_begin(sh.all, c, sh.active) > x) --c;
+    return c;
+}
+
+// CTA `cta` notes the unit whose first block is in its share and whose last is not: the pieces in between lie in the shares up to
+// the one with the unit's last block.
+__device__ __forceinline__ void note_cut(const PagedArgs& a, const Share& sh, const Segment& g, int cta, int row0, int rows, int q0) {
+    const int last = cta_of(sh, g.begin + a.start_cost + g.unit_blocks - 1);
     a.cut[2 * cta] = make_int4(g.b, g.h, row0, rows);
-    a.cut[2 * cta + 1] = make_int4(static_cast<int>(c) - cta + 1, q0, 0, 0);
+    a.cut[2 * cta + 1] = make_int4(last - cta + 1, q0, 0, 0);
 }
 
 }  // namespace ring

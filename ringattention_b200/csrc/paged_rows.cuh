@@ -96,14 +96,14 @@ __global__ void __launch_bounds__(T::kThreads) ring_paged_rows_kernel(const Page
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int cta = blockIdx.x;
     griddep_launch();  // the joining kernel may take its place; it waits for this grid's end before it reads
-    plan_start<T::BN, T::kThreads>(a, plan, cta, gridDim.x);
+    using U = AttentionUnits<T::BN>;
+    Share share;
+    Segment g = plan_start<U, T::kThreads>(a, plan, share, cta, gridDim.x);
     if (tid == 0) a.cut[2 * cta + 1] = make_int4(0, 0, 0, 0);
 
     const uint32_t ring = smem_u32(smem) + warp * T::kRing;
     const uint16_t* kbase = static_cast<const uint16_t*>(a.k);
     const uint16_t* vbase = static_cast<const uint16_t*>(a.v);
-    int64_t x = plan.x0;
-    Segment g = plan.seg;
     while (g.valid) {
         const SeqView s = seq_view(a, g.b);
         const int row0 = g.tile * T::kRows;
@@ -386,22 +386,18 @@ __global__ void __launch_bounds__(T::kThreads) ring_paged_rows_kernel(const Page
                 if (col == 0) a.lse[token * a.heads + head] = lse;
             }
         }
-        if (slot == 2 * cta + 1 && tid == 0) note_cut(a, plan, g, cta, x, row0, rows, s.q0);
-        x += g.count;
-        __syncthreads();  // the join's memory becomes rings again
-        if (tid == 0) plan.seg = plan_next<T::BN>(a, g, plan.x1 - x);
-        __syncthreads();
-        g = plan.seg;
+        if (slot == 2 * cta + 1 && tid == 0) note_cut(a, share, g, cta, row0, rows, s.q0);
+        g = plan_next<U>(a, share, g);
+        if (g.valid) __syncthreads();  // the join's memory becomes rings again
     }
 }
 
 // Joins the partials of the units that share boundaries have cut: CTA (c, y) takes rows y, y + gridDim.y, ... of the unit that
-// begins in share c.  kSplit warps take turns over the partials of one row.  Reads every partial once: bound by
-// latency at decoding sizes, which is why the warps split the list.
+// begins in share c.  out = sum_p exp(lse_p - lse) out_p with lse over all partials first, so that the loads of the
+// second pass do not wait on one another.  kSplit warps share the partials of one row.  Bound by latency.
 template <int D, bool kBf16, int kSplit>
 __global__ void __launch_bounds__(128) ring_paged_join_kernel(const PagedArgs a, int unit_rows) {
     using namespace ptx;
-    __shared__ float sm_m[4][32 / (D / 4)], sm_l[4][32 / (D / 4)];
     __shared__ float4 sm_o[4][32];
     griddep_wait();
     if (a.status && *reinterpret_cast<volatile int*>(a.status) != 0) return;  // a wait ran out: the partials are not whole
@@ -414,70 +410,67 @@ __global__ void __launch_bounds__(128) ring_paged_join_kernel(const PagedArgs a,
     constexpr int kLanes = D / 4;          // lanes per row
     constexpr int kSub = 32 / kLanes;      // partials a warp reads at once
     constexpr int kRowsAtOnce = 4 / kSplit;
+    constexpr int kPieces = kSplit * kSub;
     const int sub = lane / kLanes, col = (lane % kLanes) * 4;
-    const int piece = (warp % kSplit) * kSub + sub, pieces = kSplit * kSub;
-    for (int row = blockIdx.y * kRowsAtOnce + warp / kSplit; row - warp / kSplit < u.w; row += gridDim.y * kRowsAtOnce) {
+    const int piece = (warp % kSplit) * kSub + sub;
+    for (int r0 = blockIdx.y * kRowsAtOnce; r0 < u.w; r0 += gridDim.y * kRowsAtOnce) {
+        const int row = r0 + warp / kSplit;
         const bool live = row < u.w;
-        float mx = -INFINITY, l = 0.f;
+        auto at = [&](int p) { return static_cast<int64_t>(p == 0 ? 2 * c + 1 : 2 * (c + p)) * unit_rows + row; };
+        float lse = -INFINITY;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         if (live) {
-#pragma unroll 4
-            for (int p = piece; p < parts; p += pieces) {
-                const int slot = p == 0 ? 2 * c + 1 : 2 * (c + p);
-                const int64_t at = static_cast<int64_t>(slot) * unit_rows + row;
-                const float e = a.part_lse[at];
-                const float4 v = *reinterpret_cast<const float4*>(a.part_o + at * D + col);
+            float mx = -INFINITY, l = 0.f;
+            for (int p = lane; p < parts; p += 32) {
+                const float e = a.part_lse[at(p)];
                 const float m2 = fmaxf(mx, e);
-                const float fa = mx == m2 ? 1.f : expf(mx - m2), fb = e == -INFINITY ? 0.f : expf(e - m2);
-                acc.x = acc.x * fa + v.x * fb;
-                acc.y = acc.y * fa + v.y * fb;
-                acc.z = acc.z * fa + v.z * fb;
-                acc.w = acc.w * fa + v.w * fb;
-                l = l * fa + fb;
+                l = (mx == m2 ? l : l * expf(mx - m2)) + (e == -INFINITY ? 0.f : expf(e - m2));
                 mx = m2;
             }
-        }
-        if (pieces > 1) {
-            sm_o[warp][lane] = acc;
-            if (col == 0) {
-                sm_m[warp][sub] = mx;
-                sm_l[warp][sub] = l;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) {
+                const float m1 = __shfl_xor_sync(0xffffffffu, mx, o), l1 = __shfl_xor_sync(0xffffffffu, l, o);
+                const float m2 = fmaxf(mx, m1);
+                l = (mx == m2 ? l : l * expf(mx - m2)) + (m1 == m2 ? l1 : l1 * expf(m1 - m2));
+                mx = m2;
             }
+            if (l > 0.f || l != l) lse = (mx == -INFINITY ? 0.f : mx) + logf(l);
+#pragma unroll 8
+            for (int p = piece; p < parts; p += kPieces) {
+                const float e = a.part_lse[at(p)];
+                const float w = e == -INFINITY ? 0.f : expf(e - lse);
+                const float4 v = *reinterpret_cast<const float4*>(a.part_o + at(p) * D + col);
+                acc.x = fmaf(v.x, w, acc.x);
+                acc.y = fmaf(v.y, w, acc.y);
+                acc.z = fmaf(v.z, w, acc.z);
+                acc.w = fmaf(v.w, w, acc.w);
+            }
+        }
+        if (kPieces > 1) {
+            sm_o[warp][lane] = acc;
             __syncthreads();
             if (live && piece == 0) {
-                const int w0 = warp;  // first warp of this row
-                for (int p = 1; p < pieces; ++p) {
-                    const float e = sm_m[w0 + p / kSub][p % kSub];
-                    const float4 v = sm_o[w0 + p / kSub][(p % kSub) * kLanes + lane];
-                    const float m2 = fmaxf(mx, e);
-                    const float fa = mx == m2 ? 1.f : expf(mx - m2), fb = e == -INFINITY ? 0.f : expf(e - m2);
-                    acc.x = acc.x * fa + v.x * fb;
-                    acc.y = acc.y * fa + v.y * fb;
-                    acc.z = acc.z * fa + v.z * fb;
-                    acc.w = acc.w * fa + v.w * fb;
-                    l = l * fa + sm_l[w0 + p / kSub][p % kSub] * fb;
-                    mx = m2;
+                for (int p = 1; p < kPieces; ++p) {
+                    const float4 v = sm_o[warp + p / kSub][(p % kSub) * kLanes + lane];
+                    acc.x += v.x;
+                    acc.y += v.y;
+                    acc.z += v.z;
+                    acc.w += v.w;
                 }
             }
             __syncthreads();
         }
         if (live && piece == 0) {
-            const bool have = l > 0.f || l != l;
-            const float inv = have ? 1.f / l : 0.f;
             const int r = u.z + row, tok = r / a.group;
             const int64_t token = more.y + tok;
             const int head = u.y * a.group + (r - tok * a.group);
-            const int64_t at = token * a.out_token + head * a.out_head + col;
-            acc.x *= inv;
-            acc.y *= inv;
-            acc.z *= inv;
-            acc.w *= inv;
+            const int64_t to = token * a.out_token + head * a.out_head + col;
             if (a.out_fp32)
-                *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = acc;
+                *reinterpret_cast<float4*>(static_cast<float*>(a.out) + to) = acc;
             else
-                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) =
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + to) =
                     make_uint2(pack16<kBf16>(acc.x, acc.y), pack16<kBf16>(acc.z, acc.w));
-            if (col == 0) a.lse[token * a.heads + head] = have ? mx + logf(l) : -INFINITY;
+            if (col == 0) a.lse[token * a.heads + head] = lse;
         }
     }
 }
