@@ -116,6 +116,12 @@ void query_args(const Ring_paged_params& p, ring::PagedArgs* a) {
     a->q_head = p.q_head_stride;
     a->heads = p.heads;
     a->group = p.kv_heads ? p.heads / p.kv_heads : 0;
+    if (a->group) {
+        uint32_t shift = 0;
+        while ((1u << shift) < static_cast<uint32_t>(a->group)) ++shift;
+        a->group_shift = shift;
+        a->group_mul = static_cast<uint32_t>(((uint64_t(1) << 32) * ((uint64_t(1) << shift) - a->group)) / a->group + 1);
+    }
     a->out_fp32 = p.out_fp32;
     a->out = p.out;
     a->out_token = p.out_token_stride;
@@ -146,12 +152,14 @@ int set_smem(Kernel kernel, int bytes, bool* done) {
     return RING_OK;
 }
 
-// A launch that may begin while the kernel before it in the stream is still running (it waits for that kernel itself).
+// Every kernel here is launched so that its CTAs may be set up while the kernel before it in the stream still runs; each waits
+// (griddepcontrol.wait) for that kernel's end and its memory before it reads or writes anything.
 template <class... Params, class... Args>
-int launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, cudaStream_t stream, Args... args) {
+int launch(void (*kernel)(Params...), dim3 grid, dim3 block, int smem, cudaStream_t stream, const Args&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -192,10 +200,8 @@ int launch_rows(const ring::PagedArgs& a, const AttentionPlan& plan, DeviceState
     auto kernel = &ring::ring_paged_rows_kernel<T>;
     int rc = set_smem(kernel, T::kSmem, &st->paged_attr_set[(MT - 1) * 4 + (D == 128) * 2 + kBf16]);
     if (rc) return rc;
-    kernel<<<plan.grid, T::kThreads, T::kSmem, stream>>>(a);
-    RING_CUDA(cudaGetLastError());
-    g_launches.fetch_add(1, std::memory_order_relaxed);
-    return launch_dependent(&ring::ring_paged_join_kernel<D, kBf16, 4>, dim3(plan.grid, plan.rows), dim3(128), stream, a, plan.unit_rows);
+    if ((rc = launch(kernel, dim3(plan.grid), dim3(T::kThreads), T::kSmem, stream, a))) return rc;
+    return launch(&ring::ring_paged_join_kernel<D, kBf16, 4>, dim3(plan.grid, plan.rows), dim3(128), 0, stream, a, plan.unit_rows);
 }
 
 // The cache as a 4-D map [pages, kv_heads, page_size, dim]: a box is 64 columns of min(page_size, 128) places of one page and head,
@@ -228,10 +234,8 @@ int launch_chunk(const ring::PagedArgs& a, const AttentionPlan& plan, DeviceStat
     CUtensorMap tk, tv;
     if ((rc = cache_map(&tk, a, a.k, a.k_page, a.k_head, a.k_place, D, kBf16))) return rc;
     if ((rc = cache_map(&tv, a, a.v, a.v_page, a.v_head, a.v_place, D, kBf16))) return rc;
-    kernel<<<plan.grid, T::kNThreads, T::kSmemSize, stream>>>(tk, tv, a);
-    RING_CUDA(cudaGetLastError());
-    g_launches.fetch_add(1, std::memory_order_relaxed);
-    return launch_dependent(&ring::ring_paged_join_kernel<D, kBf16, 1>, dim3(plan.grid, 32), dim3(128), stream, a, plan.unit_rows);
+    if ((rc = launch(kernel, dim3(plan.grid), dim3(T::kNThreads), T::kSmemSize, stream, tk, tv, a))) return rc;
+    return launch(&ring::ring_paged_join_kernel<D, kBf16, 1>, dim3(plan.grid, 32), dim3(128), 0, stream, a, plan.unit_rows);
 }
 
 template <int D, bool kBf16>
@@ -247,10 +251,7 @@ int launch_weights(const ring::PagedArgs& a, DeviceState* st, cudaStream_t strea
     auto kernel = &ring::ring_paged_weights_kernel<T>;
     int rc = set_smem(kernel, T::kSmem, &st->paged_attr_set[16 + (D == 128) * 2 + kBf16]);
     if (rc) return rc;
-    kernel<<<dim3((a.capacity + T::kPlaces - 1) / T::kPlaces, a.kv_heads, a.batch), T::kThreads, T::kSmem, stream>>>(a);
-    RING_CUDA(cudaGetLastError());
-    g_launches.fetch_add(1, std::memory_order_relaxed);
-    return RING_OK;
+    return launch(kernel, dim3((a.capacity + T::kPlaces - 1) / T::kPlaces, a.kv_heads, a.batch), dim3(T::kThreads), T::kSmem, stream, a);
 }
 
 }  // namespace
@@ -291,13 +292,8 @@ int ring_paged_append(const Ring_paged_params* params) {
     PAGED_REQUIRE((warps + 7) / 8 <= kMaxInt, "too many tokens");
     const int blocks = static_cast<int>((warps + 7) / 8);
     cudaStream_t stream = static_cast<cudaStream_t>(p.stream);
-    if (p.dim == 128)
-        ring::ring_paged_append_kernel<128><<<blocks, 256, 0, stream>>>(args);
-    else
-        ring::ring_paged_append_kernel<64><<<blocks, 256, 0, stream>>>(args);
-    RING_CUDA(cudaGetLastError());
-    g_launches.fetch_add(1, std::memory_order_relaxed);
-    return RING_OK;
+    return launch(p.dim == 128 ? &ring::ring_paged_append_kernel<128> : &ring::ring_paged_append_kernel<64>, dim3(blocks), dim3(256), 0,
+                  stream, args);
 }
 
 int64_t ring_paged_attention_workspace(const Ring_paged_params* params) {
@@ -336,6 +332,7 @@ int ring_paged_attention_fwd(const Ring_paged_params* params) {
     a.part_lse = reinterpret_cast<float*>(ws + plan.o_bytes);
     a.cut = reinterpret_cast<int4*>(ws + plan.o_bytes + plan.lse_bytes);
     a.unit_rows = plan.unit_rows;
+    a.unit_shift = __builtin_ctz(static_cast<unsigned>(plan.unit_rows));
     a.many_tiles = (static_cast<int64_t>(max_new_of(p)) * a.group + plan.unit_rows - 1) / plan.unit_rows > 4;
     a.start_cost = plan.unit_rows == 256 ? 3 : 2;
     a.min_blocks = a.start_cost + (plan.unit_rows == 256 ? 2 : 1);
@@ -399,13 +396,11 @@ int ring_paged_evict(const Ring_evict_params* params) {
     e.kept = p.kept;
     e.new_lens = p.new_lens;
     cudaStream_t stream = static_cast<cudaStream_t>(p.stream);
-    ring::ring_paged_select_kernel<<<p.batch * p.kv_heads, ring::kSelectThreads, 0, stream>>>(e);
-    RING_CUDA(cudaGetLastError());
-    g_launches.fetch_add(1, std::memory_order_relaxed);
+    if ((rc = launch(&ring::ring_paged_select_kernel, dim3(p.batch * p.kv_heads), dim3(ring::kSelectThreads), 0, stream, e))) return rc;
     const int per_block = 8 * 4 * (p.dim == 128 ? 1 : 2);
     const dim3 grid((p.budget + per_block - 1) / per_block, p.batch * p.kv_heads);
-    if (p.dim == 128) return launch_dependent(&ring::ring_paged_gather_kernel<128>, grid, dim3(256), stream, e);
-    return launch_dependent(&ring::ring_paged_gather_kernel<64>, grid, dim3(256), stream, e);
+    if (p.dim == 128) return launch(&ring::ring_paged_gather_kernel<128>, grid, dim3(256), 0, stream, e);
+    return launch(&ring::ring_paged_gather_kernel<64>, grid, dim3(256), 0, stream, e);
 }
 
 }  // extern "C"

@@ -53,6 +53,7 @@ __global__ void __launch_bounds__(256) ring_paged_append_kernel(const PagedAppen
     const int t = static_cast<int>(w / p.head_parts);
     const int part = static_cast<int>(w % p.head_parts);
     if (t >= a.tokens) return;
+    ptx::griddep_wait();
     const int per = (a.kv_heads + p.head_parts - 1) / p.head_parts;
     const int h_begin = part * per, h_end = min(a.kv_heads, h_begin + per);
     const int ch = (lane % kChunks) * 8, hl = lane / kChunks;
@@ -113,6 +114,7 @@ __global__ void __launch_bounds__(T::kThreads) ring_paged_weights_kernel(const P
     constexpr int D = T::D;
     constexpr int kChunks = T::kRowBytes / 16;
     extern __shared__ __align__(128) uint8_t smem[];
+    griddep_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int h = blockIdx.y, b = blockIdx.z;
     const int j0 = blockIdx.x * T::kPlaces;
@@ -267,6 +269,7 @@ __global__ void __launch_bounds__(kSelectThreads) ring_paged_select_kernel(const
     __shared__ uint32_t hist[kSelectBins];
     __shared__ uint32_t warp_sum[32];
     __shared__ uint32_t found_digit, found_above;
+    ptx::griddep_wait();
     ptx::griddep_launch();
     const int tid = threadIdx.x;
     const int b = blockIdx.x / a.kv_heads, h = blockIdx.x % a.kv_heads;

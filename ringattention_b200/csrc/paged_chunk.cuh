@@ -75,6 +75,7 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int cta = blockIdx.x;
+    griddep_wait();    // nothing before this may touch memory
     griddep_launch();
     if (tid == 0) {
         *abort_flag = 0;
@@ -126,8 +127,8 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         rows = tile_rows(a, s, g.tile);
         ntiles = rows > 128 ? 2 : 1;
         tb = tile_blocks<BN>(a, s, row0, rows);
-        hi_max = token_hi(a, s, (row0 + rows - 1) / a.group);
-        lo_min = token_lo(a, s, row0 / a.group);
+        hi_max = token_hi(a, s, div_group(a, row0 + rows - 1));
+        lo_min = token_lo(a, s, div_group(a, row0));
     };
     // All threads meet; returns false when the CTA is through (its share is done or a wait ran out).
     auto end_segment = [&]() {
@@ -316,7 +317,7 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                         const int r = warp_row + u * kRowsPer + lane / kChunks;
                         val[u] = make_uint4(0u, 0u, 0u, 0u);
                         if (r < rows) {
-                            const int at = row0 + r, tok = at / a.group;
+                            const int at = row0 + r, tok = div_group(a, at);
                             val[u] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + static_cast<int64_t>(s.q0 + tok) * a.q_token +
                                                                      static_cast<int64_t>(g.h * a.group + (at - tok * a.group)) * a.q_head + ch * 8);
                         }
@@ -332,9 +333,9 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                 }
                 // ---- limits of this thread's row, and of the tile (for the blocks that need no mask)
                 const int row = warp_row + lane;
-                const int tok = (row0 + min(row, rows - 1)) / a.group;
+                const int tok = div_group(a, row0 + min(row, rows - 1));
                 const int hi = token_hi(a, s, tok), lo = token_lo(a, s, tok);
-                const int tile_first = (row0 + t * 128) / a.group, tile_last = (row0 + min(t * 128 + 127, rows - 1)) / a.group;
+                const int tile_first = div_group(a, row0 + t * 128), tile_last = div_group(a, row0 + min(t * 128 + 127, rows - 1));
                 const int hi_min = token_hi(a, s, tile_first), lo_max = token_lo(a, s, tile_last);
                 auto pages_of = [&](int i) {  // which pages of block i exist, a bit each
                     int have = 0;
@@ -486,7 +487,7 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                                 if (slot >= 0) {
                                     *reinterpret_cast<float4*>(a.part_o + (static_cast<int64_t>(slot) * a.unit_rows + r) * D + col) = val;
                                 } else {
-                                    const int at = row0 + r, tk = at / a.group;
+                                    const int at = row0 + r, tk = div_group(a, at);
                                     const int64_t to = static_cast<int64_t>(s.q0 + tk) * a.out_token +
                                                        static_cast<int64_t>(g.h * a.group + (at - tk * a.group)) * a.out_head + col;
                                     if (a.out_fp32)

@@ -30,13 +30,14 @@ struct PagedArgs {
     const void* q;
     int64_t q_token, q_head;
     int heads, group;  // group = heads / kv_heads
+    uint32_t group_mul, group_shift;  // x / group = (umulhi(x, mul) + x) >> shift for 0 <= x < 2^31
     int out_fp32;
     void* out;
     int64_t out_token, out_head;
     float* lse;  // [tokens, heads]
     float scale, scale_log2;
     int causal, window, sinks;
-    int unit_rows;    // query rows (token-major, then head of the group) per unit
+    int unit_rows, unit_shift;  // query rows (token-major, then head of the group) per unit, a power of two
     int many_tiles;   // hint: a sequence may have many tiles, sum its blocks with a warp instead of a thread
     int min_blocks;   // cost a CTA should at least get
     int start_cost;   // cost of starting a unit, in blocks
@@ -48,6 +49,10 @@ struct PagedArgs {
     int4* cut;  // two int4 per CTA: {sequence, kv head, first row, rows}, {parts, first token row, 0, 0}
     int* status;
 };
+
+__device__ __forceinline__ int div_group(const PagedArgs& a, int x) {
+    return static_cast<int>((__umulhi(static_cast<uint32_t>(x), a.group_mul) + static_cast<uint32_t>(x)) >> a.group_shift);
+}
 
 struct SeqView {
     int q0;   // first packed row
@@ -92,7 +97,7 @@ struct TileBlocks {
 
 template <int BN>
 __device__ __forceinline__ TileBlocks tile_blocks(const PagedArgs& a, const SeqView& s, int row0, int rows) {
-    const int t0 = row0 / a.group, t1 = (row0 + rows - 1) / a.group;
+    const int t0 = div_group(a, row0), t1 = div_group(a, row0 + rows - 1);
     const int hi = token_hi(a, s, t1), lo = token_lo(a, s, t0);
     TileBlocks r;
     r.sink = 0;
@@ -107,7 +112,7 @@ __device__ __forceinline__ TileBlocks tile_blocks(const PagedArgs& a, const SeqV
 }
 
 __device__ __forceinline__ int seq_tiles(const PagedArgs& a, const SeqView& s) {
-    return (s.n * a.group + a.unit_rows - 1) / a.unit_rows;
+    return (s.n * a.group + a.unit_rows - 1) >> a.unit_shift;
 }
 __device__ __forceinline__ int tile_rows(const PagedArgs& a, const SeqView& s, int tile) {
     return min(a.unit_rows, s.n * a.group - tile * a.unit_rows);
@@ -132,27 +137,41 @@ struct Segment {
     int64_t begin;    // where the unit begins in the list of costs
 };
 
-// A CTA's share [x0, x1) of the list of costs.
+// A CTA's share [x0, x1) of the list of costs: quot + 1 for the first rem shares, quot for the others.
 struct Share {
-    int64_t all;  // the whole list
+    int64_t quot, rem;
     int active;   // CTAs that have a share
     int64_t x0, x1;
 };
 
-__device__ __forceinline__ int64_t share_begin(int64_t all, int c, int n) {
-    if (all < (1 << 21)) return static_cast<uint32_t>(all) * static_cast<uint32_t>(c) / static_cast<uint32_t>(n);  // c, n < 2^11
-    return all * c / n;
+// List positions may pass 32 bits (a very long prompt), and a 64-bit division is a long piece of code that every launch would
+// fetch: x / n for n < 2^15 goes digit by digit, quotients by other list positions are found by halving.
+__device__ __forceinline__ int64_t div_small(int64_t x, uint32_t n) {
+    if ((x >> 32) == 0) return static_cast<uint32_t>(x) / n;
+    int64_t q = 0;
+    uint32_t r = 0;
+#pragma unroll 1
+    for (int sh = 48; sh >= 0; sh -= 16) {
+        const uint32_t cur = r << 16 | static_cast<uint32_t>((x >> sh) & 0xffff);
+        q = q << 16 | (cur / n);
+        r = cur % n;
+    }
+    return q;
 }
+
+__device__ __forceinline__ int64_t share_begin(const Share& sh, int c) { return c * sh.quot + (c < sh.rem ? c : sh.rem); }
 
 __device__ __forceinline__ Share make_share(const PagedArgs& a, int64_t all, int cta, int ctas) {
     Share r;
-    r.all = all;
-    const int64_t want = all < (1 << 30) ? static_cast<uint32_t>(all + a.min_blocks - 1) / static_cast<uint32_t>(a.min_blocks) : ctas;
-    r.active = static_cast<int>(want < ctas ? want : ctas);
-    r.x0 = r.x1 = 0;
+    r.active = all >= static_cast<int64_t>(a.min_blocks) * ctas
+                   ? ctas
+                   : (static_cast<int>(all) + a.min_blocks - 1) / a.min_blocks;
+    r.quot = r.rem = r.x0 = r.x1 = 0;
     if (cta < r.active) {
-        r.x0 = share_begin(all, cta, r.active);
-        r.x1 = share_begin(all, cta + 1, r.active);
+        r.quot = div_small(all, r.active);
+        r.rem = all - r.quot * r.active;
+        r.x0 = share_begin(r, cta);
+        r.x1 = share_begin(r, cta + 1);
     }
     return r;
 }
@@ -193,8 +212,9 @@ __device__ __forceinline__ Segment first_segment(const PagedArgs& a, const Share
     Segment g;
     g.b = b;
     const int64_t rel = sh.x0 - before;
-    g.h = rel < (1 << 30) && own < (1 << 30) ? static_cast<int>(static_cast<uint32_t>(rel) / static_cast<uint32_t>(own))
-                                              : static_cast<int>(rel / own);
+    g.h = 0;
+    for (int step = 1 << (31 - __clz(a.kv_heads)); step; step >>= 1)
+        if (g.h + step < a.kv_heads && (g.h + step) * own <= rel) g.h += step;
     g.tiles = U::tiles(a, s);
     int64_t at = before + g.h * own;  // list position of the tiles looked at
     g.tile = 0;
@@ -351,18 +371,18 @@ __device__ __forceinline__ int partial_slot(const Segment& g, int cta) {
     return g.first > 0 ? 2 * cta : 2 * cta + 1;
 }
 
-// The CTA whose share holds list position x.
-__device__ __forceinline__ int cta_of(const Share& sh, int64_t x) {
-    int c = static_cast<int>(x * sh.active / sh.all);
-    while (c + 1 < sh.active && share_begin(sh.all, c + 1, sh.active) <= x) ++c;
-    while (c > 0 && share_begin(sh.all, c, sh.active) > x) --c;
+// The CTA, `cta` or a later one, whose share holds list position x.
+__device__ __forceinline__ int cta_of(const Share& sh, int cta, int64_t x) {
+    int c = cta;
+    for (int step = 1 << (31 - __clz(sh.active)); step; step >>= 1)
+        if (c + step < sh.active && share_begin(sh, c + step) <= x) c += step;
     return c;
 }
 
 // CTA `cta` notes the unit whose first block is in its share and whose last is not: the pieces in between lie in the shares up to
 // the one with the unit's last block.
 __device__ __forceinline__ void note_cut(const PagedArgs& a, const Share& sh, const Segment& g, int cta, int row0, int rows, int q0) {
-    const int last = cta_of(sh, g.begin + a.start_cost + g.unit_blocks - 1);
+    const int last = cta_of(sh, cta, g.begin + a.start_cost + g.unit_blocks - 1);
     a.cut[2 * cta] = make_int4(g.b, g.h, row0, rows);
     a.cut[2 * cta + 1] = make_int4(last - cta + 1, q0, 0, 0);
 }

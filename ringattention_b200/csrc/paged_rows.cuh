@@ -85,31 +85,52 @@ struct PagedRowsTraits {
 template <class T>
 __global__ void __launch_bounds__(T::kThreads) ring_paged_rows_kernel(const PagedArgs a) {
     using namespace ptx;
+    using U = AttentionUnits<T::BN>;
     constexpr int D = T::D, MT = T::MT, KT = T::KT;
     constexpr int kChunks = T::kRowBytes / 16;       // 16-byte chunks per row
     constexpr int kRowsPer = 32 / kChunks;           // rows one warp-wide cp.async covers
     constexpr int kLoads = KT / kRowsPer;            // ... per K or V of a step (8)
     constexpr int NG = KT / 8;                       // groups of 8 places (a page holds whole groups)
+    constexpr int kBatch = 32 / NG;                  // steps whose page ids one warp-wide load fetches
+    constexpr int kAhead = T::kStages - 1;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ PlanShared plan;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int cta = blockIdx.x;
+    griddep_wait();    // nothing before this may touch memory
     griddep_launch();  // the joining kernel may take its place; it waits for this grid's end before it reads
-    using U = AttentionUnits<T::BN>;
     Share share;
     Segment g = plan_start<U, T::kThreads>(a, plan, share, cta, gridDim.x);
     if (tid == 0) a.cut[2 * cta + 1] = make_int4(0, 0, 0, 0);
 
     const uint32_t ring = smem_u32(smem) + warp * T::kRing;
-    const uint16_t* kbase = static_cast<const uint16_t*>(a.k);
-    const uint16_t* vbase = static_cast<const uint16_t*>(a.v);
+    const int page_mask = (1 << a.page_shift) - 1;
+    // Steps of this warp: warp, warp + 4, ... of the segment's, KT places each.  D = 128: sub-block `warp` of block i; D = 64:
+    // half warp & 1 of block 2 i + (warp >> 1).
+    auto steps_of = [&](const Segment& sg) { return (sg.count * T::kSteps - warp + T::kWarps - 1) / T::kWarps; };
+    auto place_of = [&](const Segment& sg, const TileBlocks& tb, int i) {
+        const int st = warp + i * T::kWarps;
+        return tb.block(sg.first + st / T::kSteps) * T::BN + (st % T::kSteps) * KT;
+    };
+    // Page ids of steps [kBatch * n, kBatch * (n + 1)): lane l has group l % NG of step l / NG, -1 where there is none.
+    auto load_pages = [&](const Segment& sg, const TileBlocks& tb, int n) {
+        const int i = n * kBatch + lane / NG;
+        if (i >= steps_of(sg)) return -1;
+        return page_of(a, sg.b, (place_of(sg, tb, i) + 8 * (lane % NG)) >> a.page_shift);
+    };
+    SeqView s;
+    TileBlocks tb;
+    int ids = -1;
+    if (g.valid) {
+        s = seq_view(a, g.b);
+        tb = tile_blocks<T::BN>(a, s, g.tile * T::kRows, tile_rows(a, s, g.tile));
+        ids = load_pages(g, tb, 0);
+    }
     while (g.valid) {
-        const SeqView s = seq_view(a, g.b);
         const int row0 = g.tile * T::kRows;
         const int rows = tile_rows(a, s, g.tile);
-        const TileBlocks tb = tile_blocks<T::BN>(a, s, row0, rows);
-        const int tok_first = row0 / a.group, tok_last = (row0 + rows - 1) / a.group;
+        const int tok_first = div_group(a, row0), tok_last = div_group(a, row0 + rows - 1);
         const int hi_max = token_hi(a, s, tok_last), hi_min = token_hi(a, s, tok_first);
         const int lo_min = token_lo(a, s, tok_first), lo_max = token_lo(a, s, tok_last);
 
@@ -123,7 +144,7 @@ __global__ void __launch_bounds__(T::kThreads) ring_paged_rows_kernel(const Page
             for (int r = 0; r < 2; ++r) {
                 const int row = 16 * m + 8 * r + (lane >> 2);
                 const int at = row0 + min(row, rows - 1);
-                const int tok = at / a.group;
+                const int tok = div_group(a, at);
                 qp[r] = static_cast<const uint16_t*>(a.q) + static_cast<int64_t>(s.q0 + tok) * a.q_token +
                         static_cast<int64_t>(g.h * a.group + (at - tok * a.group)) * a.q_head + 2 * (lane & 3);
                 hi[m][r] = row < rows ? token_hi(a, s, tok) : 0;
@@ -151,64 +172,59 @@ __global__ void __launch_bounds__(T::kThreads) ring_paged_rows_kernel(const Page
             l_run[m][0] = l_run[m][1] = 0.f;
         }
 
-        // ---- this warp's steps of the segment: step i covers KT places from place_of(i)
-        const int steps = g.count * T::kSteps;
-        const int mine = (steps - warp + T::kWarps - 1) / T::kWarps;  // steps warp, warp + 4, ...
-        auto place_of = [&](int i) {
-            const int st = warp + i * T::kWarps;
-            return tb.block(g.first + st / T::kSteps) * T::BN + (st % T::kSteps) * KT;
-        };
-        // page of the lane's group (lanes 0..NG-1) of step i
-        auto load_pages = [&](int i) {
-            int id = -1;
-            if (i < mine && lane < NG) id = page_of(a, g.b, (place_of(i) + 8 * lane) >> a.page_shift);
-            return id;
-        };
-        const int64_t khead = static_cast<int64_t>(g.h) * a.k_head + (lane % kChunks) * 8;
-        const int64_t vhead = static_cast<int64_t>(g.h) * a.v_head + (lane % kChunks) * 8;
-        const int page_mask = (1 << a.page_shift) - 1;
-        auto fill = [&](int i, int ids) {
-            const uint32_t dst = ring + (i % T::kStages) * T::kStageBytes;
-            const int j0 = place_of(i);
-#pragma unroll
-            for (int u = 0; u < kLoads; ++u) {
-                const int r = u * kRowsPer + lane / kChunks;
-                const int id = __shfl_sync(0xffffffffu, ids, (u * kRowsPer) / 8);
-                const int j = j0 + r;
-                const bool ok = id >= 0 && j < hi_max && (j >= lo_min || j < a.sinks);
-                const int64_t pg = ok ? id : 0, sl = ok ? (j & page_mask) : 0;
-                const uint32_t to = dst + r * T::kRowBytes + (((lane % kChunks) ^ (r & 7)) << 4);
-                cp_async16(to, kbase + pg * a.k_page + sl * a.k_place + khead, ok);
-                cp_async16(to + T::kHalf, vbase + pg * a.v_page + sl * a.v_place + vhead, ok);
-            }
-        };
-        int ids_next = load_pages(0);
-        int seen[T::kStages];  // bit per group of 8 places: its page exists
-#pragma unroll
-        for (int i = 0; i < T::kStages - 1; ++i) {
-            const int ids = ids_next;
-            ids_next = load_pages(i + 1);
-            seen[i] = __ballot_sync(0xffffffffu, ids >= 0);
-            if (i < mine) fill(i, ids);
-            cp_async_commit();
-        }
-
+        const int mine = steps_of(g);
+        // this lane's part of every K and V address
+        const uint16_t* kl = static_cast<const uint16_t*>(a.k) + static_cast<int64_t>(g.h) * a.k_head + (lane % kChunks) * 8 + (lane / kChunks) * a.k_place;
+        const uint16_t* vl = static_cast<const uint16_t*>(a.v) + static_cast<int64_t>(g.h) * a.v_head + (lane % kChunks) * 8 + (lane / kChunks) * a.v_place;
+        int ids_next = -1;
+        uint32_t have = 0;       // bit l: lane l's id of the current batch exists
+        uint32_t seen = 0;       // NG bits per stage, the step being computed lowest: its groups' pages exist
+        // The loop runs kAhead steps early to fill the ring: one copy of the code, and of its instruction fetches.
 #pragma unroll 1
-        for (int i = 0; i < mine; ++i) {
-            {  // refill the stage freed by the previous step
-                const int n = i + T::kStages - 1;
-                const int ids = ids_next;
-                ids_next = load_pages(n + 1);
-                seen[T::kStages - 1] = __ballot_sync(0xffffffffu, ids >= 0);
-                __syncwarp();
-                if (n < mine) fill(n, ids);
-                cp_async_commit();
+        for (int i = -kAhead; i < mine; ++i) {
+            const int n = i + kAhead;
+            if (n < mine) {
+                if (n % kBatch == 0) {
+                    if (n > 0) ids = ids_next;
+                    ids_next = load_pages(g, tb, n / kBatch + 1);
+                    have = __ballot_sync(0xffffffffu, ids >= 0);
+                }
+                const int j0 = place_of(g, tb, n);
+                const uint32_t bits = (have >> ((n % kBatch) * NG)) & ((1u << NG) - 1u);
+                seen |= bits << (kAhead * NG);
+                const bool inside = j0 + KT <= hi_max && (j0 >= lo_min || j0 + KT <= a.sinks);
+                const uint32_t dst = ring + (n % T::kStages) * T::kStageBytes + (lane / kChunks) * T::kRowBytes;
+                __syncwarp();  // every lane is done with the stage
+#pragma unroll
+                for (int gr = 0; gr < NG; ++gr) {
+                    const int id = __shfl_sync(0xffffffffu, ids, (n % kBatch) * NG + gr);
+                    const int64_t pg = id >= 0 ? id : 0;
+                    const int slot = (j0 + 8 * gr) & page_mask;
+                    const uint16_t* kp = kl + pg * a.k_page + static_cast<int64_t>(slot) * a.k_place;
+                    const uint16_t* vp = vl + pg * a.v_page + static_cast<int64_t>(slot) * a.v_place;
+#pragma unroll
+                    for (int u = 0; u < 8 / kRowsPer; ++u) {
+                        const int r = gr * 8 + u * kRowsPer;  // + lane / kChunks
+                        const int j = j0 + r + lane / kChunks;
+                        const bool ok = id >= 0 && (inside || (j < hi_max && (j >= lo_min || j < a.sinks)));
+                        const uint32_t to = dst + r * T::kRowBytes + (((lane % kChunks) ^ ((u * kRowsPer + lane / kChunks) & 7)) << 4);
+                        cp_async16(to, kp, ok);
+                        cp_async16(to + T::kHalf, vp, ok);
+                        kp += kRowsPer * a.k_place;
+                        vp += kRowsPer * a.v_place;
+                    }
+                }
             }
-            cp_async_wait<T::kStages - 1>();
+            cp_async_commit();
+            if (i < 0) {
+                seen >>= NG;
+                continue;
+            }
+            cp_async_wait<kAhead>();
             __syncwarp();
             const uint32_t kst = ring + (i % T::kStages) * T::kStageBytes;
             const uint32_t vst = kst + T::kHalf;
-            const int j0 = place_of(i);
+            const int j0 = place_of(g, tb, i);
 
             // S = Q K^T: KT / 8 fragments of 16 rows x 8 places
             float sc[MT][NG][4];
@@ -234,7 +250,7 @@ __global__ void __launch_bounds__(T::kThreads) ring_paged_rows_kernel(const Page
                 }
             }
 
-            const bool edge = j0 + KT > hi_min || lo_max > j0 || (seen[0] & ((1 << NG) - 1)) != (1 << NG) - 1;
+            const bool edge = j0 + KT > hi_min || lo_max > j0 || (seen & ((1u << NG) - 1u)) != (1u << NG) - 1u;
             if (edge) {
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
@@ -243,12 +259,11 @@ __global__ void __launch_bounds__(T::kThreads) ring_paged_rows_kernel(const Page
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int j = j0 + 8 * n + 2 * (lane & 3) + (e & 1);
-                            const bool see = j < hi[m][e >> 1] && (j >= lo[m][e >> 1] || j < a.sinks) && ((seen[0] >> n) & 1);
+                            const bool see = j < hi[m][e >> 1] && (j >= lo[m][e >> 1] || j < a.sinks) && ((seen >> n) & 1u);
                             if (!see) sc[m][n][e] = -INFINITY;
                         }
             }
-#pragma unroll
-            for (int st = 0; st + 1 < T::kStages; ++st) seen[st] = seen[st + 1];
+            seen >>= NG;
 
             uint32_t pf[MT][NG][2];  // P as A fragments
 #pragma unroll
@@ -315,7 +330,15 @@ __global__ void __launch_bounds__(T::kThreads) ring_paged_rows_kernel(const Page
                     }
                 }
             }
-            __syncwarp();  // the stage may be refilled
+        }
+        // the next segment's lookups travel while this one's warps are joined
+        const Segment g_next = plan_next<U>(a, share, g);
+        SeqView s_next = s;
+        TileBlocks tb_next = tb;
+        if (g_next.valid) {
+            if (g_next.b != g.b) s_next = seq_view(a, g_next.b);
+            tb_next = tile_blocks<T::BN>(a, s_next, g_next.tile * T::kRows, tile_rows(a, s_next, g_next.tile));
+            ids = load_pages(g_next, tb_next, 0);
         }
         cp_async_wait<0>();
         __syncthreads();  // every warp is done with its ring: the join overlays them
@@ -373,7 +396,7 @@ __global__ void __launch_bounds__(T::kThreads) ring_paged_rows_kernel(const Page
                 *reinterpret_cast<float4*>(a.part_o + at * D + col) = acc;
                 if (col == 0) a.part_lse[at] = lse;
             } else {
-                const int r = row0 + row, tok = r / a.group;
+                const int r = row0 + row, tok = div_group(a, r);
                 const int64_t token = s.q0 + tok;
                 const int head = g.h * a.group + (r - tok * a.group);
                 const int64_t at = token * a.out_token + head * a.out_head + col;
@@ -387,7 +410,9 @@ __global__ void __launch_bounds__(T::kThreads) ring_paged_rows_kernel(const Page
             }
         }
         if (slot == 2 * cta + 1 && tid == 0) note_cut(a, share, g, cta, row0, rows, s.q0);
-        g = plan_next<U>(a, share, g);
+        g = g_next;
+        s = s_next;
+        tb = tb_next;
         if (g.valid) __syncthreads();  // the join's memory becomes rings again
     }
 }
@@ -461,7 +486,7 @@ __global__ void __launch_bounds__(128) ring_paged_join_kernel(const PagedArgs a,
             __syncthreads();
         }
         if (live && piece == 0) {
-            const int r = u.z + row, tok = r / a.group;
+            const int r = u.z + row, tok = div_group(a, r);
             const int64_t token = more.y + tok;
             const int head = u.y * a.group + (r - tok * a.group);
             const int64_t to = token * a.out_token + head * a.out_head + col;
