@@ -258,7 +258,7 @@ int ring_static_status(int* status_out, void* stream);
  *
  * Cache.  K and V live in `num_pages` pages of `page_size` places per K/V head.  A place is a row of `dim` contiguous
  * elements; pages, heads and places may be laid out in any order (strides in elements, multiples of 8, bases 16-byte
- * aligned), so both [pages, kv_heads, page_size, dim] and [pages, page_size, kv_heads, dim] are served.  page_size is a
+ * aligned, no two rows one memory), so both [pages, kv_heads, page_size, dim] and [pages, page_size, kv_heads, dim] are served.  page_size is a
  * power of two >= 8.
  * Sequences.  page_table[b * table_stride + i] (device, int32) names the page holding places [i, i + 1) * page_size of
  * sequence b; kv_lens[b] (device, int32) is its length in places INCLUDING this step's new tokens.  An id outside
@@ -309,7 +309,7 @@ typedef struct Ring_paged_params {
     int64_t weights_batch_stride, weights_head_stride;
     int weights_len; /* >= max_pages * page_size */
     int is_bf16;
-    /* ring_paged_attention_fwd: scratch of at least ring_paged_attention_workspace() bytes, 256-byte aligned */
+    /* attention and weights: scratch of at least ring_paged_{attention,weights}_workspace() bytes, 256-byte aligned */
     void* workspace;
     int64_t workspace_bytes;
     void* stream;
@@ -339,6 +339,8 @@ int64_t ring_paged_attention_workspace(const Ring_paged_params* params);
  * Every place is added to by one thread in a fixed order: the result does not depend on timing.  Asynchronous on `stream`.
  */
 int ring_paged_weights(const Ring_paged_params* params);
+/* Scratch bytes of ring_paged_weights for these sizes (0: none is needed), or a negative RingStatus. */
+int64_t ring_paged_weights_workspace(const Ring_paged_params* params);
 
 /*
  * Eviction by accumulated attention weight.  Of the len places of sequence b, m = min(len, budget) stay, for every K/V head

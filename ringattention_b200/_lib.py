@@ -115,6 +115,7 @@ SYMBOLS = {
     "ring_paged_append": (c_int, [ctypes.POINTER(Ring_paged_params)]),
     "ring_paged_attention_fwd": (c_int, [ctypes.POINTER(Ring_paged_params)]),
     "ring_paged_attention_workspace": (c_int64, [ctypes.POINTER(Ring_paged_params)]),
+    "ring_paged_weights_workspace": (c_int64, [ctypes.POINTER(Ring_paged_params)]),
     "ring_paged_weights": (c_int, [ctypes.POINTER(Ring_paged_params)]),
     "ring_paged_evict": (c_int, [ctypes.POINTER(Ring_evict_params)]),
     "ring_device_status": (c_int, [ctypes.POINTER(c_int)]),

@@ -23,7 +23,7 @@ __all__ = [
     "ring_attention", "ring_attention_scaled", "set_params_fprop", "Ring_fwd_params", "RingContext",
     "attention_block_fwd", "lse_merge", "device_status", "device_status_reset", "kernel_launch_count",
     "attention_chunked_fwd_static", "static_status",
-    "paged_append", "paged_attention_fwd", "paged_attention_workspace", "paged_weights", "paged_evict",
+    "paged_append", "paged_attention_fwd", "paged_attention_workspace", "paged_weights", "paged_weights_workspace", "paged_evict",
 ]
 
 
@@ -409,6 +409,20 @@ def _on(device, stream):
     return ctx, _stream_handle(stream)
 
 
+def _workspace(p, size, workspace, device, where: str):
+    """The caller's scratch, or one from torch's allocator for the stream the call goes to, so that the allocator orders the
+    memory's next user behind this call."""
+    import torch
+    if workspace is None:
+        n = size(ctypes.byref(p))
+        if n < 0:
+            check(int(n), where)
+        with torch.cuda.stream(torch.cuda.ExternalStream(p.stream, device) if p.stream else torch.cuda.default_stream(device)):
+            workspace = torch.empty(int(n), dtype=torch.uint8, device=device)
+    p.workspace, _ = _strided(workspace, "workspace", 1, (torch.uint8,), device)
+    p.workspace_bytes = workspace.numel()
+
+
 def paged_append(k, v, k_cache, v_cache, page_table, kv_lens, *, cu_seqlens=None, weights=None, stream=None) -> None:
     """Write the new tokens' rows k, v [tokens, kv_heads, dim] to their places in the pages.
 
@@ -433,18 +447,27 @@ def paged_append(k, v, k_cache, v_cache, page_table, kv_lens, *, cu_seqlens=None
         check(_lib.load().ring_paged_append(ctypes.byref(p)), "ring_paged_append")
 
 
-def paged_attention_workspace(q, k_cache, page_table, *, cu_seqlens=None, max_new: int = 0) -> int:
-    """Bytes of scratch paged_attention_fwd needs for tensors of these shapes (independent of what they hold)."""
+def _workspace_bytes(name: str, q, k_cache, page_table, cu_seqlens, max_new) -> int:
+    import torch
     p = _lib.Ring_paged_params()
     p.kv_heads, p.dim, p.heads, p.softmax_scale = k_cache.shape[1], k_cache.shape[3], q.shape[1], 1.0
     p.batch, p.max_pages = page_table.shape
     _fill_tokens(p, q.shape[0], cu_seqlens, max_new, k_cache.device)
-    import torch
     with torch.cuda.device(k_cache.device):
-        n = _lib.load().ring_paged_attention_workspace(ctypes.byref(p))
+        n = getattr(_lib.load(), name)(ctypes.byref(p))
     if n < 0:
-        check(int(n), "ring_paged_attention_workspace")
+        check(int(n), name)
     return int(n)
+
+
+def paged_attention_workspace(q, k_cache, page_table, *, cu_seqlens=None, max_new: int = 0) -> int:
+    """Bytes of scratch paged_attention_fwd needs for tensors of these shapes (independent of what they hold)."""
+    return _workspace_bytes("ring_paged_attention_workspace", q, k_cache, page_table, cu_seqlens, max_new)
+
+
+def paged_weights_workspace(q, k_cache, page_table, *, cu_seqlens=None, max_new: int = 0) -> int:
+    """Bytes of scratch paged_weights needs for tensors of these shapes; 0: none."""
+    return _workspace_bytes("ring_paged_weights_workspace", q, k_cache, page_table, cu_seqlens, max_new)
 
 
 def paged_attention_fwd(q, k_cache, v_cache, page_table, kv_lens, out, lse, *, cu_seqlens=None, max_new: int = 0,
@@ -472,23 +495,15 @@ def paged_attention_fwd(q, k_cache, v_cache, page_table, kv_lens, out, lse, *, c
     ctx, p.stream = _on(dev, stream)
     with ctx:
         lib = _lib.load()
-        if workspace is None:
-            n = lib.ring_paged_attention_workspace(ctypes.byref(p))
-            if n < 0:
-                check(int(n), "ring_paged_attention_fwd")
-            # allocated for the stream the call goes to, so that the allocator orders its next user behind this call
-            with torch.cuda.stream(torch.cuda.ExternalStream(p.stream, dev) if p.stream else torch.cuda.default_stream(dev)):
-                workspace = torch.empty(n, dtype=torch.uint8, device=dev)
-        p.workspace, _ = _strided(workspace, "workspace", 1, (torch.uint8,), dev)
-        p.workspace_bytes = workspace.numel()
+        _workspace(p, lib.ring_paged_attention_workspace, workspace, dev, "ring_paged_attention_fwd")
         check(lib.ring_paged_attention_fwd(ctypes.byref(p)), "ring_paged_attention_fwd")
 
 
 def paged_weights(weights, q, k_cache, lse, page_table, kv_lens, *, cu_seqlens=None, max_new: int = 0,
-                  softmax_scale: Optional[float] = None, causal: bool = True, window: int = 0, sinks: int = 0, stream=None) -> None:
+                  softmax_scale: Optional[float] = None, causal: bool = True, window: int = 0, sinks: int = 0, workspace=None, stream=None) -> None:
     """weights [batch, kv_heads, places] fp32 += the attention that every cached place received from the new tokens: exp(s - lse)
     summed over the tokens that see it and the query heads of its K/V head, with the lse of paged_attention_fwd for the same
-    arguments.  places >= max_pages * page_size."""
+    arguments.  places >= max_pages * page_size.  workspace as for paged_attention_fwd, of paged_weights_workspace() bytes."""
     p = _lib.Ring_paged_params()
     _fill_cache(p, k_cache, None, page_table, kv_lens)
     _fill_queries(p, q, k_cache, lse, softmax_scale, causal, window, sinks)
@@ -497,7 +512,9 @@ def paged_weights(weights, q, k_cache, lse, page_table, kv_lens, *, cu_seqlens=N
     _distinct(weights, "weights")
     ctx, p.stream = _on(k_cache.device, stream)
     with ctx:
-        check(_lib.load().ring_paged_weights(ctypes.byref(p)), "ring_paged_weights")
+        lib = _lib.load()
+        _workspace(p, lib.ring_paged_weights_workspace, workspace, k_cache.device, "ring_paged_weights")
+        check(lib.ring_paged_weights(ctypes.byref(p)), "ring_paged_weights")
 
 
 def paged_evict(k_cache, v_cache, weights, page_table, kv_lens, dst_table, budget: int, new_lens, new_weights, kept, *,

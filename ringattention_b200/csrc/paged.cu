@@ -16,6 +16,7 @@
 #include "paged_chunk.cuh"
 #include "paged_plan.cuh"
 #include "paged_rows.cuh"
+#include "paged_weights.cuh"
 
 using namespace ring_host;
 
@@ -102,6 +103,7 @@ int check_queries(const Ring_paged_params& p, bool pointers) {
         PAGED_REQUIRE(aligned16(p.q), "q must be 16-byte aligned");
         PAGED_REQUIRE(((p.q_token_stride | p.q_head_stride) & 7) == 0 && p.q_token_stride >= 0 && p.q_head_stride >= 0,
                       "q strides must be non-negative multiples of 8 elements");
+        PAGED_REQUIRE((p.tokens == 1 || p.q_token_stride) && (p.heads == 1 || p.q_head_stride), "q strides of 0 (an expanded tensor) are not supported");
     }
     return RING_OK;
 }
@@ -168,6 +170,12 @@ int launch(void (*kernel)(Params...), dim3 grid, dim3 block, int smem, cudaStrea
     cfg.numAttrs = 1;
     RING_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
     g_launches.fetch_add(1, std::memory_order_relaxed);
+    return RING_OK;
+}
+
+int check_workspace(const Ring_paged_params& p, int64_t need) {
+    PAGED_REQUIRE(p.workspace && (reinterpret_cast<uintptr_t>(p.workspace) & 255) == 0, "workspace must be 256-byte aligned and not null");
+    PAGED_REQUIRE(p.workspace_bytes >= need, "workspace holds %lld bytes, %lld are needed", (long long)p.workspace_bytes, (long long)need);
     return RING_OK;
 }
 
@@ -245,13 +253,78 @@ int launch_attention(const ring::PagedArgs& a, const AttentionPlan& plan, Device
     return launch_rows<D, kBf16, 2>(a, plan, st, stream);
 }
 
-template <int D, bool kBf16>
-int launch_weights(const ring::PagedArgs& a, DeviceState* st, cudaStream_t stream) {
-    using T = ring::PagedWeightsTraits<D, kBf16>;
-    auto kernel = &ring::ring_paged_weights_kernel<T>;
-    int rc = set_smem(kernel, T::kSmem, &st->paged_attr_set[16 + (D == 128) * 2 + kBf16]);
+// ---- weights -------------------------------------------------------------------------------------------------------
+struct WeightsPlan {
+    bool chunk;      // many query rows: the tcgen05 form
+    int row_tiles;   // rows form: tiles of 8 query rows held in registers
+    int grid;
+    int64_t part_bytes, cut_bytes;
+    int64_t bytes() const { return part_bytes + cut_bytes; }
+};
+
+WeightsPlan weights_plan(const Ring_paged_params& p, int sm_count) {
+    WeightsPlan r;
+    const int64_t group = p.heads / p.kv_heads, rows = max_new_of(p) * group;
+    r.chunk = rows > 32 && group <= 128;  // a query tile of the chunk form holds whole tokens of at most 128 heads
+    r.row_tiles = rows <= 8 ? 1 : (rows <= 16 ? 2 : 4);
+    r.grid = r.chunk ? sm_count : 2 * sm_count;
+    r.part_bytes = r.chunk ? round256(int64_t(2) * r.grid * 256 * 4) : 0;
+    r.cut_bytes = r.chunk ? round256(int64_t(r.grid) * 32) : 0;
+    return r;
+}
+
+template <int D, bool kBf16, int NT>
+int launch_weights_rows(const ring::PagedArgs& a, const WeightsPlan& plan, DeviceState* st, cudaStream_t stream) {
+    using T = ring::PagedWeightsRowsTraits<D, kBf16, NT>;
+    auto kernel = &ring::ring_paged_weights_rows_kernel<T>;
+    int rc = set_smem(kernel, T::kSmem, &st->paged_attr_set[16 + (NT >> 1) * 4 + (D == 128) * 2 + kBf16]);
     if (rc) return rc;
-    return launch(kernel, dim3((a.capacity + T::kPlaces - 1) / T::kPlaces, a.kv_heads, a.batch), dim3(T::kThreads), T::kSmem, stream, a);
+    return launch(kernel, dim3(plan.grid), dim3(T::kThreads), T::kSmem, stream, a);
+}
+
+// The queries as a 4-D map [tokens, kv_heads, group, dim]: a box is 64 columns of all heads of a group for `row_tokens` tokens.
+int query_map(CUtensorMap* tm, const ring::PagedArgs& a, int dim, bool bf16) {
+    EncodeTiledFn enc = nullptr;
+    int rc = encode_fn(&enc);
+    if (rc) return rc;
+    const int64_t head = a.heads == 1 ? dim : a.q_head, token = a.tokens == 1 ? dim : a.q_token;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(a.group), static_cast<cuuint64_t>(a.kv_heads),
+                                static_cast<cuuint64_t>(a.tokens)};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(head) * 2, static_cast<cuuint64_t>(head) * a.group * 2, static_cast<cuuint64_t>(token) * 2};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(a.group), 1, static_cast<cuuint32_t>(a.row_tokens)};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    const CUresult r = enc(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(a.q), dims,
+                           strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(RING_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+    return RING_OK;
+}
+
+template <int D, bool kBf16>
+int launch_weights(const ring::PagedArgs& a, const WeightsPlan& plan, DeviceState* st, cudaStream_t stream) {
+    if (!plan.chunk) {
+        if (plan.row_tiles == 1) return launch_weights_rows<D, kBf16, 1>(a, plan, st, stream);
+        if (plan.row_tiles == 2) return launch_weights_rows<D, kBf16, 2>(a, plan, st, stream);
+        return launch_weights_rows<D, kBf16, 4>(a, plan, st, stream);
+    }
+    using T = ring::PagedWeightsTraits<D, typename std::conditional<kBf16, __nv_bfloat16, __half>::type>;
+    auto kernel = &ring::ring_paged_weights_chunk_kernel<T>;
+    int rc = set_smem(kernel, T::kSmemSize, &st->paged_attr_set[12 + (D == 128) * 2 + kBf16]);
+    if (rc) return rc;
+    CUtensorMap tk, tq;
+    if ((rc = cache_map(&tk, a, a.k, a.k_page, a.k_head, a.k_place, D, kBf16))) return rc;
+    if ((rc = query_map(&tq, a, D, kBf16))) return rc;
+    if ((rc = launch(kernel, dim3(plan.grid), dim3(T::kNThreads), T::kSmemSize, stream, tk, tq, a))) return rc;
+    return launch(&ring::ring_paged_weights_join_kernel, dim3(plan.grid), dim3(256), 0, stream, a);
+}
+
+// What the workspace questions look at.
+int check_sizes(const Ring_paged_params* params, DeviceState** st) {
+    if (!params) return fail(RING_ERR_INVALID_ARGUMENT, "null params");
+    PAGED_REQUIRE(params->dim == 64 || params->dim == 128, "dim must be 64 or 128, got %d", params->dim);
+    PAGED_REQUIRE(params->batch >= 1 && params->kv_heads >= 1, "batch and kv_heads must be positive");
+    const int rc = check_queries(*params, false);
+    return rc ? rc : device_state(st);
 }
 
 }  // namespace
@@ -297,15 +370,15 @@ int ring_paged_append(const Ring_paged_params* params) {
 }
 
 int64_t ring_paged_attention_workspace(const Ring_paged_params* params) {
-    if (!params) return fail(RING_ERR_INVALID_ARGUMENT, "null params");
-    const Ring_paged_params& p = *params;
-    PAGED_REQUIRE(p.dim == 64 || p.dim == 128, "dim must be 64 or 128, got %d", p.dim);
-    PAGED_REQUIRE(p.batch >= 1 && p.kv_heads >= 1, "batch and kv_heads must be positive");
-    int rc = check_queries(p, false);
-    if (rc) return rc;
     DeviceState* st = nullptr;
-    if ((rc = device_state(&st))) return rc;
-    return attention_plan(p, st->sm_count).bytes();
+    const int rc = check_sizes(params, &st);
+    return rc ? rc : attention_plan(*params, st->sm_count).bytes();
+}
+
+int64_t ring_paged_weights_workspace(const Ring_paged_params* params) {
+    DeviceState* st = nullptr;
+    const int rc = check_sizes(params, &st);
+    return rc ? rc : weights_plan(*params, st->sm_count).bytes();
 }
 
 int ring_paged_attention_fwd(const Ring_paged_params* params) {
@@ -322,9 +395,7 @@ int ring_paged_attention_fwd(const Ring_paged_params* params) {
     DeviceState* st = nullptr;
     if ((rc = device_state(&st))) return rc;
     const AttentionPlan plan = attention_plan(p, st->sm_count);
-    PAGED_REQUIRE(p.workspace && (reinterpret_cast<uintptr_t>(p.workspace) & 255) == 0, "workspace must be 256-byte aligned and not null");
-    PAGED_REQUIRE(p.workspace_bytes >= plan.bytes(), "workspace holds %lld bytes, %lld are needed", (long long)p.workspace_bytes,
-                  (long long)plan.bytes());
+    if ((rc = check_workspace(p, plan.bytes()))) return rc;
     ring::PagedArgs a;
     query_args(p, &a);
     char* ws = static_cast<char*>(p.workspace);
@@ -354,9 +425,22 @@ int ring_paged_weights(const Ring_paged_params* params) {
     if ((rc = device_state(&st))) return rc;
     ring::PagedArgs a;
     query_args(p, &a);
+    const WeightsPlan plan = weights_plan(p, st->sm_count);
+    if (plan.bytes() > 0) {
+        if ((rc = check_workspace(p, plan.bytes()))) return rc;
+        a.part_lse = static_cast<float*>(p.workspace);
+        a.cut = reinterpret_cast<int4*>(static_cast<char*>(p.workspace) + plan.part_bytes);
+    }
+    a.status = st->d_status;
+    a.row_tokens = plan.chunk ? 128 / a.group : 0;
+    a.unit_rows = 1 << 30;  // one unit holds all rows of its sequence
+    a.unit_shift = 30;
+    a.many_tiles = plan.chunk;
+    a.start_cost = 1;
+    a.min_blocks = 2;
     cudaStream_t stream = static_cast<cudaStream_t>(p.stream);
-    if (p.dim == 128) return p.is_bf16 ? launch_weights<128, true>(a, st, stream) : launch_weights<128, false>(a, st, stream);
-    return p.is_bf16 ? launch_weights<64, true>(a, st, stream) : launch_weights<64, false>(a, st, stream);
+    if (p.dim == 128) return p.is_bf16 ? launch_weights<128, true>(a, plan, st, stream) : launch_weights<128, false>(a, plan, st, stream);
+    return p.is_bf16 ? launch_weights<64, true>(a, plan, st, stream) : launch_weights<64, false>(a, plan, st, stream);
 }
 
 int ring_paged_evict(const Ring_evict_params* params) {

@@ -1,4 +1,4 @@
-// Paged-cache kernels that move rows: append and eviction, and the simple form of the accumulated attention weights.
+// Paged-cache kernels that move rows: append and eviction.
 #pragma once
 
 #include <cstdint>
@@ -92,122 +92,6 @@ __global__ void __launch_bounds__(256) ring_paged_append_kernel(const PagedAppen
                 if (a.weights && ch == 0) a.weights[b * a.w_batch + h * a.w_head + place] = 0.f;
             }
         }
-    }
-}
-
-// ------------------------------------------------------------------------------------------------ attention weights
-// Accumulated attention weights: one CTA per 64 places of one K/V head, S^T = K Q^T with the places as the rows of the product (mma.sync
-// m16n8k16), p = exp2(s c - lse log2 e) summed over the query rows in registers.  No atomics: a place belongs to one
-// thread's sum, in the order of the rows.
-template <int D_, bool kBf16_>
-struct PagedWeightsTraits {
-    static constexpr int D = D_;
-    static constexpr bool kBf16 = kBf16_;
-    static constexpr int kPlaces = 64, kThreads = 128, kQRows = 64;
-    static constexpr int kRowBytes = D * 2;
-    static constexpr int kSmem = (kPlaces + kQRows) * kRowBytes + kQRows * 12;
-};
-
-template <class T>
-__global__ void __launch_bounds__(T::kThreads) ring_paged_weights_kernel(const PagedArgs a) {
-    using namespace ptx;
-    constexpr int D = T::D;
-    constexpr int kChunks = T::kRowBytes / 16;
-    extern __shared__ __align__(128) uint8_t smem[];
-    griddep_wait();
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int h = blockIdx.y, b = blockIdx.z;
-    const int j0 = blockIdx.x * T::kPlaces;
-    const SeqView s = seq_view(a, b);
-    if (j0 >= s.len || s.n == 0) return;
-    // tokens that see a place of this tile
-    int t_begin = 0, t_end = s.n;
-    if (a.causal) t_begin = max(0, j0 - (s.len - s.n));
-    if (a.window > 0 && j0 >= a.sinks) t_end = static_cast<int>(min(static_cast<int64_t>(s.n), static_cast<int64_t>(j0) + T::kPlaces - 1 + a.window - (s.len - s.n)));
-    if (t_begin >= t_end) return;
-
-    const uint32_t sk = smem_u32(smem), sq = sk + T::kPlaces * T::kRowBytes;
-    float* lse2 = reinterpret_cast<float*>(smem + (T::kPlaces + T::kQRows) * T::kRowBytes);
-    int* his = reinterpret_cast<int*>(lse2 + T::kQRows);
-    int* los = his + T::kQRows;
-    const int page_mask = (1 << a.page_shift) - 1;
-    const int hi_max = token_hi(a, s, s.n - 1);
-    for (int i = tid; i < T::kPlaces * kChunks; i += T::kThreads) {
-        const int r = i / kChunks, c = i % kChunks, j = j0 + r;
-        const int id = j < hi_max ? page_of(a, b, j >> a.page_shift) : -1;
-        const bool ok = id >= 0;
-        const uint16_t* src = static_cast<const uint16_t*>(a.k) + (ok ? id : 0) * a.k_page + (ok ? (j & page_mask) : 0) * a.k_place +
-                              h * a.k_head + c * 8;
-        cp_async16(sk + r * T::kRowBytes + ((c ^ (r & 7)) << 4), src, ok);
-    }
-    cp_async_commit();
-
-    uint32_t kf[D / 16][4];
-    float w[2] = {0.f, 0.f};
-    const int j_lo = j0 + warp * 16 + (lane >> 2);
-    const int row_end = t_end * a.group;
-    bool first = true;
-    for (int r0 = t_begin * a.group; r0 < row_end; r0 += T::kQRows) {
-        if (!first) __syncthreads();
-        for (int i = tid; i < T::kQRows * kChunks; i += T::kThreads) {
-            const int r = i / kChunks, c = i % kChunks;
-            const bool ok = r0 + r < row_end;
-            const int at = ok ? r0 + r : r0;
-            const int tok = at / a.group;
-            const uint16_t* src = static_cast<const uint16_t*>(a.q) + static_cast<int64_t>(s.q0 + tok) * a.q_token +
-                                  static_cast<int64_t>(h * a.group + (at - tok * a.group)) * a.q_head + c * 8;
-            cp_async16(sq + r * T::kRowBytes + ((c ^ (r & 7)) << 4), src, ok);
-        }
-        cp_async_commit();
-        if (tid < T::kQRows) {
-            const bool ok = r0 + tid < row_end;
-            const int at = ok ? r0 + tid : r0;
-            const int tok = at / a.group;
-            const float l = a.lse[static_cast<int64_t>(s.q0 + tok) * a.heads + h * a.group + (at - tok * a.group)];
-            lse2[tid] = (ok && l != -INFINITY) ? l * 1.4426950408889634f : INFINITY;
-            his[tid] = ok ? token_hi(a, s, tok) : 0;
-            los[tid] = token_lo(a, s, tok);
-        }
-        cp_async_wait<0>();
-        __syncthreads();
-        if (first) {
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-                const int r = warp * 16 + (lane & 15), c = 2 * kk + (lane >> 4);
-                ldmatrix_x4(kf[kk], sk + r * T::kRowBytes + ((c ^ (r & 7)) << 4));
-            }
-            first = false;
-        }
-        const int n_rows = min(T::kQRows, row_end - r0);
-        for (int n = 0; n < n_rows; n += 16) {
-            float sc[2][4] = {};
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-                uint32_t qf[4];
-                const int r = n + (lane & 7) + ((lane >> 4) << 3), c = 2 * kk + ((lane >> 3) & 1);
-                ldmatrix_x4(qf, sq + r * T::kRowBytes + ((c ^ (r & 7)) << 4));
-                mma_16816<T::kBf16>(sc[0], kf[kk], qf[0], qf[1]);
-                mma_16816<T::kBf16>(sc[1], kf[kk], qf[2], qf[3]);
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = n + 8 * u + 2 * (lane & 3) + (e & 1);
-                    const int j = j_lo + 8 * (e >> 1);
-                    const bool see = j < his[r] && (j >= los[r] || j < a.sinks);
-                    const float p = ex2_approx(fmaf(sc[u][e], a.scale_log2, -lse2[r]));
-                    w[e >> 1] += see ? p : 0.f;
-                }
-        }
-    }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        w[e] += __shfl_xor_sync(0xffffffffu, w[e], 1);
-        w[e] += __shfl_xor_sync(0xffffffffu, w[e], 2);
-        const int j = j_lo + 8 * e;
-        if ((lane & 3) == 0 && j < hi_max && page_of(a, b, j >> a.page_shift) >= 0)
-            a.weights[b * a.w_batch + h * a.w_head + j] += w[e];
     }
 }
 

@@ -43,7 +43,9 @@ struct PagedArgs {
     int start_cost;   // cost of starting a unit, in blocks
     float* weights;
     int64_t w_batch, w_head;
-    // workspace of the attention kernels: part_o [2 * grid][unit_rows][D], part_lse [2 * grid][unit_rows], cut [grid]
+    int row_tokens;   // weights, chunk form: tokens per tile of query rows
+    // workspace.  Attention: part_o [2 * grid][unit_rows][D], part_lse [2 * grid][unit_rows], cut [grid];
+    // weights, chunk form: part_lse [2 * grid][256] (sums), cut [grid]
     float* part_o;
     float* part_lse;
     int4* cut;  // two int4 per CTA: {sequence, kv head, first row, rows}, {parts, first token row, 0, 0}

@@ -8,6 +8,8 @@
 #include <torch/extension.h>
 
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <vector>
@@ -196,6 +198,16 @@ void fill_queries(Ring_paged_params& p, const at::Tensor& q, const at::Tensor& k
     p.is_bf16 = q.scalar_type() == at::kBFloat16 ? 1 : 0;
 }
 
+// Scratch from torch's allocator for the current stream: calls that overlap get memory of their own, and nothing is kept.
+c10::DataPtr take_workspace(Ring_paged_params& p, int64_t bytes, const char* what) {
+    TORCH_CHECK(bytes >= 0, what, " failed (", bytes, "): ", ring_last_error_string());
+    if (bytes == 0) return {};
+    c10::DataPtr w = c10::cuda::CUDACachingAllocator::get()->allocate(static_cast<size_t>(bytes));
+    p.workspace = w.get();
+    p.workspace_bytes = bytes;
+    return w;
+}
+
 void paged_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache,
                   const at::Tensor& page_table, const at::Tensor& kv_lens, const c10::optional<at::Tensor>& cu_seqlens,
                   const c10::optional<at::Tensor>& weights) {
@@ -218,28 +230,23 @@ void paged_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_
     check_status(ring_paged_append(&p), "ring_paged_append");
 }
 
-std::vector<at::Tensor> paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
-                                        const at::Tensor& page_table, const at::Tensor& kv_lens,
-                                        const c10::optional<at::Tensor>& cu_seqlens, int64_t max_new,
+std::tuple<at::Tensor, at::Tensor> paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                                   const at::Tensor& page_table, const at::Tensor& kv_lens,
+                                                   const c10::optional<at::Tensor>& cu_seqlens, int64_t max_new,
                                         const c10::optional<double>& softmax_scale, bool causal, int64_t window, int64_t sinks, bool fp32_out) {
     Ring_paged_params p{};
     fill_cache(p, k_cache, &v_cache, page_table, kv_lens);
     fill_queries(p, q, k_cache, softmax_scale, causal, window, sinks);
     fill_tokens(p, q.size(0), cu_seqlens, max_new, k_cache.device());
     const c10::cuda::CUDAGuard guard(k_cache.device());
-    auto out = at::empty(q.sizes(), q.options().dtype(fp32_out ? at::kFloat : q.scalar_type()));
-    auto lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+    at::Tensor out(at::detail::empty_cuda(q.sizes(), fp32_out ? at::kFloat : q.scalar_type(), q.device(), c10::nullopt));
+    at::Tensor lse(at::detail::empty_cuda({q.size(0), q.size(1)}, at::kFloat, q.device(), c10::nullopt));
     p.out = out.data_ptr();
     p.out_token_stride = out.stride(0);
     p.out_head_stride = out.stride(1);
     p.out_fp32 = fp32_out ? 1 : 0;
     p.lse = lse.data_ptr<float>();
-    const int64_t bytes = ring_paged_attention_workspace(&p);
-    TORCH_CHECK(bytes >= 0, "ring_paged_attention_fwd failed (", bytes, "): ", ring_last_error_string());
-    // from torch's allocator on this stream: calls that overlap get memory of their own, and nothing is kept
-    auto workspace = at::empty({bytes}, q.options().dtype(at::kByte));
-    p.workspace = workspace.data_ptr();
-    p.workspace_bytes = bytes;
+    const c10::DataPtr workspace = take_workspace(p, ring_paged_attention_workspace(&p), "ring_paged_attention_fwd");
     check_status(ring_paged_attention_fwd(&p), "ring_paged_attention_fwd");
     return {out, lse};
 }
@@ -256,10 +263,11 @@ void paged_weights_(const at::Tensor& weights, const at::Tensor& q, const at::Te
     TORCH_CHECK(lse.is_contiguous() && lse.size(0) == q.size(0) && lse.size(1) == q.size(1), "lse must be a contiguous [tokens, heads]");
     p.lse = lse.data_ptr<float>();
     const c10::cuda::CUDAGuard guard(k_cache.device());
+    const c10::DataPtr workspace = take_workspace(p, ring_paged_weights_workspace(&p), "ring_paged_weights");
     check_status(ring_paged_weights(&p), "ring_paged_weights");
 }
 
-std::vector<at::Tensor> paged_evict(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& weights,
+std::tuple<at::Tensor, at::Tensor, at::Tensor> paged_evict(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& weights,
                                     const at::Tensor& page_table, const at::Tensor& kv_lens, const at::Tensor& dst_table, int64_t budget,
                                     int64_t first, int64_t recent) {
     Ring_evict_params p{};
@@ -283,9 +291,9 @@ std::vector<at::Tensor> paged_evict(const at::Tensor& k_cache, const at::Tensor&
     const int64_t places = dst_table.size(1) * p.page_size;
     TORCH_CHECK(budget >= 1 && budget <= places, "budget must be positive and fit the pages of dst_table (", places, " places), got ", budget);
     const c10::cuda::CUDAGuard guard(k_cache.device());
-    auto new_lens = at::empty({p.batch}, kv_lens.options());
-    auto new_weights = at::empty({p.batch, p.kv_heads, places}, weights.options());
-    auto kept = at::empty({p.batch, p.kv_heads, budget}, kv_lens.options());
+    at::Tensor new_lens(at::detail::empty_cuda({p.batch}, at::kInt, k_cache.device(), c10::nullopt));
+    at::Tensor new_weights(at::detail::empty_cuda({p.batch, p.kv_heads, places}, at::kFloat, k_cache.device(), c10::nullopt));
+    at::Tensor kept(at::detail::empty_cuda({p.batch, p.kv_heads, budget}, at::kInt, k_cache.device(), c10::nullopt));
     p.new_lens = new_lens.data_ptr<int>();
     p.new_weights = new_weights.data_ptr<float>();
     p.new_weights_batch_stride = new_weights.stride(0);

@@ -73,8 +73,8 @@ def paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens=None, m
     and the first `sinks`.  out has q's type, or fp32 with fp32_out: the partials of several caches then join with
     lse_merge_.  max_new bounds the new tokens of one sequence when cu_seqlens is given.  softmax_scale None: 1/sqrt(dim).
     """
-    return tuple(_load().paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens, max_new, softmax_scale, causal,
-                                         window, sinks, fp32_out))
+    return _load().paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens, max_new, softmax_scale, causal, window, sinks,
+                                   fp32_out)
 
 
 def paged_weights_(weights, q, k_cache, lse, page_table, kv_lens, cu_seqlens=None, max_new: int = 0,
@@ -91,4 +91,4 @@ def paged_evict(k_cache, v_cache, weights, page_table, kv_lens, dst_table, budge
     Returns (new_lens [batch] int32, new_weights [batch, kv_heads, dst places] fp32, kept [batch, kv_heads, budget] int32,
     ascending, -1 behind the last).
     """
-    return tuple(_load().paged_evict(k_cache, v_cache, weights, page_table, kv_lens, dst_table, budget, first, recent))
+    return _load().paged_evict(k_cache, v_cache, weights, page_table, kv_lens, dst_table, budget, first, recent)

@@ -78,7 +78,7 @@ def test_every_call_refuses_a_bad_cache(lib, fn, kw, needle):
     ("ring_paged_attention_fwd", dict(window=-1), "window"), ("ring_paged_attention_fwd", dict(sinks=-1), "sinks"),
     ("ring_paged_attention_fwd", dict(window=8, causal=0), "causal"), ("ring_paged_attention_fwd", dict(q=None), "null q"),
     ("ring_paged_attention_fwd", dict(lse=None), "lse"), ("ring_paged_attention_fwd", dict(q=0x5002), "aligned"),
-    ("ring_paged_attention_fwd", dict(q_head_stride=20), "multiples of 8"), ("ring_paged_attention_fwd", dict(out=None), "out"),
+    ("ring_paged_attention_fwd", dict(q_head_stride=20), "multiples of 8"), ("ring_paged_weights", dict(q_head_stride=0), "strides of 0"), ("ring_paged_attention_fwd", dict(out=None), "out"),
     ("ring_paged_attention_fwd", dict(out_token_stride=12), "out strides"), ("ring_paged_attention_fwd", dict(v_cache=None), "v_cache"),
     ("ring_paged_attention_fwd", dict(tokens=1 << 30, heads=4), "2^31"),
     ("ring_paged_weights", dict(weights=None), "null weights"), ("ring_paged_weights", dict(weights_len=10), "weights_len"),
@@ -105,7 +105,8 @@ def test_evict_refuses(lib, kw, needle):
 
 
 def test_null_params_and_workspace(lib):
-    for fn in ("ring_paged_append", "ring_paged_attention_fwd", "ring_paged_weights", "ring_paged_evict", "ring_paged_attention_workspace"):
+    for fn in ("ring_paged_append", "ring_paged_attention_fwd", "ring_paged_weights", "ring_paged_evict", "ring_paged_attention_workspace",
+               "ring_paged_weights_workspace"):
         assert getattr(lib, fn)(None) == _lib.RING_ERR_INVALID_ARGUMENT
     assert lib.ring_paged_attention_workspace(ctypes.byref(paged(dim=32))) == _lib.RING_ERR_INVALID_ARGUMENT
 

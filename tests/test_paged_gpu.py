@@ -43,6 +43,9 @@ CASES = {
     "prompt_g1": ([130, 257], [130, 257], dict(group=1, kv_heads=3, page=64)),
     "chunk_g4_d128": ([700, 300, 129], [150, 64, 129], dict(group=4, dim=128, dtype="bf16", page=128)),
     "chunk_g7": ([515, 40], [131, 40], dict(group=7, kv_heads=1, layout="NHD", page=32, dim=128)),
+    "chunk_g40": ([300, 90], [30, 11], dict(kv_heads=1, group=40, dtype="bf16")),
+    "chunk_g130": ([200], [3], dict(kv_heads=1, group=130, page=32)),
+    "long_chunk": ([5000, 1300], [700, 33], dict(kv_heads=1, group=2, page=64, dtype="bf16")),
     "page_above_tile": ([900, 513], [70, 200], dict(group=2, page=512, dim=128)),
 }
 
@@ -229,8 +232,20 @@ def test_weights(ops, name, mask):
     assert torch.equal(again, s.weights)  # the same bits again
 
 
-def test_weights_ignore_unseen_places(ops):
-    lens, news, kw = CASES["chunk_g4_d128"]
+@pytest.mark.parametrize("name", ["decode_d128_g4", "few_tokens_g5", "chunk_g4_d128", "nothing_new_for_some"])
+@pytest.mark.parametrize("hint", [1, 3, 0])
+def test_weights_hint(ops, name, hint):
+    lens, news, kw = CASES[name]
+    s = Setup(lens, news, seed=31, **kw)
+    lse = attention_ref(s)[1].float().cuda()
+    want, tol = weights_ref(s, lse)
+    ops.paged_weights_(s.weights, s.q, s.k_cache, lse, s.table, s.kv_lens, cu_seqlens=s.cu, max_new=hint)
+    assert bool(((s.weights.cpu().double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("name", ["few_tokens_g5", "chunk_g4_d128", "chunk_g7"])
+def test_weights_ignore_unseen_places(ops, name):
+    lens, news, kw = CASES[name]
     s = Setup(lens, news, seed=9, **kw)
     lse = attention_ref(s)[1].float().cuda()
     want, tol = weights_ref(s, lse)
@@ -238,7 +253,11 @@ def test_weights_ignore_unseen_places(ops):
         pg, slot = int(s.table[b, s.lens[b] // s.page]) if s.lens[b] % s.page else -1, s.lens[b] % s.page
         if pg >= 0:
             s.k_cache[pg, :, slot:] = math.nan
-    ops.paged_weights_(s.weights, s.q, s.k_cache, lse, s.table, s.kv_lens, cu_seqlens=s.cu, max_new=s.max_new)
+    for pg in s.free:
+        s.k_cache[pg] = math.nan
+    q = torch.cat([s.q, torch.full_like(s.q[:9], math.nan)])  # rows behind the last sequence
+    lse = torch.cat([lse, torch.full_like(lse[:9], math.nan)])
+    ops.paged_weights_(s.weights, q, s.k_cache, lse, s.table, s.kv_lens, cu_seqlens=s.cu, max_new=s.max_new)
     assert bool(((s.weights.cpu().double() - want).abs() <= tol).all())
 
 
@@ -444,7 +463,9 @@ def test_plain_api_matches_front_end(ops):
     w1, w2 = s.weights.clone(), s.weights.clone()
     ops.paged_weights_(w1, s.q, s.k_cache, lse, s.table, s.kv_lens, cu_seqlens=s.cu, max_new=s.max_new)
     torch.cuda.synchronize()
-    ra.paged_weights(w2, s.q, s.k_cache, lse, s.table, s.kv_lens, cu_seqlens=s.cu, max_new=s.max_new, stream=st)
+    n = ra.paged_weights_workspace(s.q, s.k_cache, s.table, cu_seqlens=s.cu, max_new=s.max_new)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    ra.paged_weights(w2, s.q, s.k_cache, lse, s.table, s.kv_lens, cu_seqlens=s.cu, max_new=s.max_new, stream=st, workspace=ws)
     st.synchronize()
     assert torch.equal(w1, w2)
     k1, k2 = s.k_cache.clone(), s.k_cache.clone()
