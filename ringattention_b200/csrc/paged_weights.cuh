@@ -251,8 +251,9 @@ struct PagedWeightsTraits : public Ring_kernel_traits<kHeadDim_, 256, 128, 12, e
     static constexpr int kQSlots = kHeadDim == 128 ? 2 : 4;
     static constexpr int kSmemTiles = (2 * kKSlots + kQSlots) * kTileBytes;
     static constexpr int kRowInfo = kQRows * 12;              // negated lse (base 2), upper and lower limit of each row
-    static constexpr int kNumBarriers = 2 * kKSlots + 2 * kQSlots + 4 /*s_full*/ + 4 /*s_free*/;
-    static constexpr int kSmemSize = kSmemTiles + kQSlots * kRowInfo + 1024 /*alignment slack*/ + 256 /*barriers, TMEM slot, flags*/;
+    static constexpr int kInfoSlots = 4;                      // a ring of its own: read until a block's sums are done, long after its tile
+    static constexpr int kNumBarriers = 2 * kKSlots + 2 * kQSlots + 4 /*s_full*/ + 4 /*s_free*/ + 2 * kInfoSlots;
+    static constexpr int kSmemSize = kSmemTiles + kInfoSlots * kRowInfo + 1024 /*alignment slack*/ + 256 /*barriers, TMEM slot, flags*/;
     static_assert(kNumBarriers * 8 + 16 <= 256 && kSmemSize <= 226 * 1024, "shared memory");
 };
 
@@ -287,7 +288,7 @@ ring_paged_weights_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const 
     const uint32_t raw_addr = smem_u32(smem_raw);
     const uint32_t base = (raw_addr + 1023u) & ~1023u;
     uint8_t* smem = smem_raw + (base - raw_addr);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + T::kSmemTiles + T::kQSlots * T::kRowInfo);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + T::kSmemTiles + T::kInfoSlots * T::kRowInfo);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + T::kNumBarriers);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* prior_error = reinterpret_cast<volatile int*>(tmem_slot + 2);
@@ -298,6 +299,8 @@ ring_paged_weights_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const 
     auto bar_q_empty = [&](int q) { return bar0 + 8u * (2 * T::kKSlots + T::kQSlots + q); };
     auto bar_s_full = [&](int m, int buf) { return bar0 + 8u * (2 * T::kKSlots + 2 * T::kQSlots + 2 * m + buf); };
     auto bar_s_free = [&](int m, int buf) { return bar0 + 8u * (2 * T::kKSlots + 2 * T::kQSlots + 4 + 2 * m + buf); };
+    auto bar_i_full = [&](int q) { return bar0 + 8u * (2 * T::kKSlots + 2 * T::kQSlots + 8 + q); };
+    auto bar_i_empty = [&](int q) { return bar0 + 8u * (2 * T::kKSlots + 2 * T::kQSlots + 8 + T::kInfoSlots + q); };
     auto smem_k = [&](int k, int m) { return base + static_cast<uint32_t>((2 * k + m) * T::kTileBytes); };
     auto smem_q = [&](int q) { return base + static_cast<uint32_t>((2 * T::kKSlots + q) * T::kTileBytes); };
     auto row_info = [&](int q) { return reinterpret_cast<float*>(smem + T::kSmemTiles + q * T::kRowInfo); };
@@ -316,8 +319,12 @@ ring_paged_weights_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const 
             mbar_init(bar_k_empty(k), 2);       // both issuers
         }
         for (int q = 0; q < T::kQSlots; ++q) {
-            mbar_init(bar_q_full(q), 2);        // the TMA transaction and the row warp
-            mbar_init(bar_q_empty(q), 2 + 8);   // both issuers (the tile) and the summing warps (the row information)
+            mbar_init(bar_q_full(q), 1);
+            mbar_init(bar_q_empty(q), 2);
+        }
+        for (int q = 0; q < T::kInfoSlots; ++q) {
+            mbar_init(bar_i_full(q), 1);        // the row warp
+            mbar_init(bar_i_empty(q), 8);       // the summing warps
         }
         for (int m = 0; m < 2; ++m)
             for (int buf = 0; buf < 2; ++buf) {
@@ -409,7 +416,7 @@ ring_paged_weights_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const 
                 U::range(a, s, g.tile, &j0, &q_first, &q_count);
 #pragma unroll 1
                 for (int i = 0; i < g.count && ok; ++i, ++blocks) {
-                    const int q = blocks % T::kQSlots;
+                    const int q = blocks % T::kInfoSlots;
                     const int t0 = (q_first + g.first + i) * a.row_tokens;
                     float nl[4];
                     int tok[4];
@@ -425,8 +432,8 @@ ring_paged_weights_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const 
                             tok[u] = -1;
                         }
                     }
-                    if (blocks >= T::kQSlots) {
-                        ok = mbar_wait(bar_q_empty(q), (blocks / T::kQSlots - 1) & 1, abort_flag, a.status, kDevPagedLoad);
+                    if (blocks >= T::kInfoSlots) {
+                        ok = mbar_wait(bar_i_empty(q), (blocks / T::kInfoSlots - 1) & 1, abort_flag, a.status, kDevPagedLoad);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
                     }
@@ -439,7 +446,7 @@ ring_paged_weights_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const 
                         reinterpret_cast<int*>(info)[2 * T::kQRows + r] = tok[u] >= 0 ? token_lo(a, s, tok[u]) : 0;
                     }
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(bar_q_full(q));
+                    if (lane == 0) mbar_arrive(bar_i_full(q));
                 }
             }
         } else {
@@ -485,8 +492,8 @@ ring_paged_weights_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const 
             float a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
 #pragma unroll 1
             for (int i = 0; i < g.count; ++i, ++blocks) {
-                const int q = blocks % T::kQSlots, buf = blocks & 1;
-                ok = mbar_wait(bar_q_full(q), (blocks / T::kQSlots) & 1, abort_flag, a.status, kDevPagedSoftmaxS) &&
+                const int q = blocks % T::kInfoSlots, buf = blocks & 1;
+                ok = mbar_wait(bar_i_full(q), (blocks / T::kInfoSlots) & 1, abort_flag, a.status, kDevPagedSoftmaxS) &&
                      mbar_wait(bar_s_full(m, buf), (blocks / 2) & 1, abort_flag, a.status, kDevPagedSoftmaxS);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
@@ -532,7 +539,7 @@ ring_paged_weights_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const 
                     }
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar_q_empty(q));
+                if (lane == 0) mbar_arrive(bar_i_empty(q));
             }
             if (!ok) break;
             const float w = (a0 + a1) + (a2 + a3);
