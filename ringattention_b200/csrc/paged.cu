@@ -108,6 +108,13 @@ int check_queries(const Ring_paged_params& p, bool pointers) {
     return RING_OK;
 }
 
+// x / d = (umulhi(x, mul) + x) >> shift for 0 <= x < 2^31: mul = floor(2^32 (2^shift - d) / d) + 1 with 2^shift >= d the least such.
+void quotient_of(int d, uint32_t* mul, uint32_t* shift) {
+    *shift = 0;
+    while ((uint64_t(1) << *shift) < static_cast<uint64_t>(d)) ++*shift;
+    *mul = static_cast<uint32_t>((uint64_t(1) << 32) * ((uint64_t(1) << *shift) - d) / d + 1);
+}
+
 void query_args(const Ring_paged_params& p, ring::PagedArgs* a) {
     cache_args(p, a);
     a->cu = p.cu_seqlens;
@@ -118,12 +125,7 @@ void query_args(const Ring_paged_params& p, ring::PagedArgs* a) {
     a->q_head = p.q_head_stride;
     a->heads = p.heads;
     a->group = p.kv_heads ? p.heads / p.kv_heads : 0;
-    if (a->group) {
-        uint32_t shift = 0;
-        while ((1u << shift) < static_cast<uint32_t>(a->group)) ++shift;
-        a->group_shift = shift;
-        a->group_mul = static_cast<uint32_t>(((uint64_t(1) << 32) * ((uint64_t(1) << shift) - a->group)) / a->group + 1);
-    }
+    if (a->group) quotient_of(a->group, &a->group_mul, &a->group_shift);
     a->out_fp32 = p.out_fp32;
     a->out = p.out;
     a->out_token = p.out_token_stride;
@@ -432,7 +434,10 @@ int ring_paged_weights(const Ring_paged_params* params) {
         a.cut = reinterpret_cast<int4*>(static_cast<char*>(p.workspace) + plan.part_bytes);
     }
     a.status = st->d_status;
-    a.row_tokens = plan.chunk ? 128 / a.group : 0;
+    if (plan.chunk) {
+        a.row_tokens = 128 / a.group;
+        quotient_of(a.row_tokens, &a.tokens_mul, &a.tokens_shift);
+    }
     a.unit_rows = 1 << 30;  // one unit holds all rows of its sequence
     a.unit_shift = 30;
     a.many_tiles = plan.chunk;

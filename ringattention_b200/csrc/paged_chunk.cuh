@@ -75,12 +75,9 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int cta = blockIdx.x;
-    griddep_wait();    // nothing before this may touch memory
     griddep_launch();
     if (tid == 0) {
         *abort_flag = 0;
-        *prior_error = *reinterpret_cast<volatile int*>(a.status);
-        a.cut[2 * cta + 1] = make_int4(0, 0, 0, 0);
         for (int t = 0; t < 2; ++t) {
             mbar_init(bar_q_full(t), 4);  // one arrival per softmax warp
             mbar_init(bar_s_full(t), 1);
@@ -97,6 +94,11 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     if (warp == T::kLoadWarp && lane == 0) {
         prefetch_tensormap(&tm_k);
         prefetch_tensormap(&tm_v);
+    }
+    griddep_wait();  // nothing before this touches memory
+    if (tid == 0) {
+        *prior_error = *reinterpret_cast<volatile int*>(a.status);
+        a.cut[2 * cta + 1] = make_int4(0, 0, 0, 0);
     }
     __syncthreads();
     if (*prior_error != 0) return;  // an earlier launch failed: do nothing (CTA-uniform)

@@ -44,6 +44,7 @@ struct PagedArgs {
     float* weights;
     int64_t w_batch, w_head;
     int row_tokens;   // weights, chunk form: tokens per tile of query rows
+    uint32_t tokens_mul, tokens_shift;  // x / row_tokens, as group_mul
     // workspace.  Attention: part_o [2 * grid][unit_rows][D], part_lse [2 * grid][unit_rows], cut [grid];
     // weights, chunk form: part_lse [2 * grid][256] (sums), cut [grid]
     float* part_o;
@@ -54,6 +55,10 @@ struct PagedArgs {
 
 __device__ __forceinline__ int div_group(const PagedArgs& a, int x) {
     return static_cast<int>((__umulhi(static_cast<uint32_t>(x), a.group_mul) + static_cast<uint32_t>(x)) >> a.group_shift);
+}
+
+__device__ __forceinline__ int div_tokens(const PagedArgs& a, int x) {
+    return static_cast<int>((__umulhi(static_cast<uint32_t>(x), a.tokens_mul) + static_cast<uint32_t>(x)) >> a.tokens_shift);
 }
 
 struct SeqView {

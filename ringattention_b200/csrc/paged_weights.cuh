@@ -250,7 +250,8 @@ struct PagedWeightsTraits : public Ring_kernel_traits<kHeadDim_, 256, 128, 12, e
     static constexpr int kKSlots = 2;                         // the next unit's places load while this one's are used
     static constexpr int kQSlots = kHeadDim == 128 ? 2 : 4;
     static constexpr int kSmemTiles = (2 * kKSlots + kQSlots) * kTileBytes;
-    static constexpr int kRowInfo = kQRows * 12;              // negated lse (base 2), upper and lower limit of each row
+    static constexpr int kRowInfo = kQRows * 4;               // negated lse (base 2) of each row
+    static constexpr int kPolyEvery = 8;                      // of 8 columns 2 are evaluated on the FMA pipe
     static constexpr int kInfoSlots = 4;                      // a ring of its own: read until a block's sums are done, long after its tile
     static constexpr int kNumBarriers = 2 * kKSlots + 2 * kQSlots + 4 /*s_full*/ + 4 /*s_free*/ + 2 * kInfoSlots;
     static constexpr int kSmemSize = kSmemTiles + kInfoSlots * kRowInfo + 1024 /*alignment slack*/ + 256 /*barriers, TMEM slot, flags*/;
@@ -266,8 +267,8 @@ struct WeightsChunkUnits {
         if (a.causal) t0 = max(0, *j0 - (s.len - s.n));
         if (a.window > 0 && *j0 >= a.sinks)
             t1 = static_cast<int>(min(static_cast<int64_t>(s.n), static_cast<int64_t>(*j0) + 255 + a.window - (s.len - s.n)));
-        *first = min(t0, s.n - 1) / a.row_tokens;
-        *count = max((t1 + a.row_tokens - 1) / a.row_tokens - *first, 1);
+        *first = div_tokens(a, min(t0, s.n - 1));
+        *count = max(div_tokens(a, max(t1, 0) + a.row_tokens - 1) - *first, 1);
     }
     static __device__ __forceinline__ int blocks(const PagedArgs& a, const SeqView& s, int tile) {
         int j0, first, count;
@@ -308,12 +309,9 @@ ring_paged_weights_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int cta = blockIdx.x;
     const int used_rows = a.row_tokens * a.group;  // rows of a query tile that hold (token, head) pairs
-    griddep_wait();    // nothing before this may touch memory
     griddep_launch();
     if (tid == 0) {
         *abort_flag = 0;
-        *prior_error = *reinterpret_cast<volatile int*>(a.status);
-        a.cut[2 * cta + 1] = make_int4(0, 0, 0, 0);
         for (int k = 0; k < T::kKSlots; ++k) {
             mbar_init(bar_k_full(k), 1);
             mbar_init(bar_k_empty(k), 2);       // both issuers
@@ -342,6 +340,11 @@ ring_paged_weights_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const 
     if (warp == T::kLoadWarp && lane == 0) {
         prefetch_tensormap(&tm_k);
         prefetch_tensormap(&tm_q);
+    }
+    griddep_wait();  // nothing before this touches memory
+    if (tid == 0) {
+        *prior_error = *reinterpret_cast<volatile int*>(a.status);
+        a.cut[2 * cta + 1] = make_int4(0, 0, 0, 0);
     }
     __syncthreads();
     if (*prior_error != 0) return;  // an earlier launch failed: do nothing (CTA-uniform)
@@ -419,17 +422,13 @@ ring_paged_weights_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const 
                     const int q = blocks % T::kInfoSlots;
                     const int t0 = (q_first + g.first + i) * a.row_tokens;
                     float nl[4];
-                    int tok[4];
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {  // the loads do not wait for the slot
                         const int r = lane + 32 * u, dt = div_group(a, r);
-                        tok[u] = t0 + dt;
-                        nl[u] = -INFINITY;
-                        if (r < used_rows && tok[u] < s.n) {
-                            const float l = a.lse[static_cast<int64_t>(s.q0 + tok[u]) * a.heads + g.h * a.group + (r - dt * a.group)];
+                        nl[u] = -INFINITY;  // rows that see nothing (lse = -inf) and rows behind the last add exp2(-inf) = 0
+                        if (r < used_rows && t0 + dt < s.n) {
+                            const float l = a.lse[static_cast<int64_t>(s.q0 + t0 + dt) * a.heads + g.h * a.group + (r - dt * a.group)];
                             if (l != -INFINITY) nl[u] = -l * 1.4426950408889634f;
-                        } else {
-                            tok[u] = -1;
                         }
                     }
                     if (blocks >= T::kInfoSlots) {
@@ -439,12 +438,7 @@ ring_paged_weights_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const 
                     }
                     float* info = row_info(q);
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const int r = lane + 32 * u;
-                        info[r] = nl[u];
-                        reinterpret_cast<int*>(info)[T::kQRows + r] = tok[u] >= 0 ? token_hi(a, s, tok[u]) : 0;
-                        reinterpret_cast<int*>(info)[2 * T::kQRows + r] = tok[u] >= 0 ? token_lo(a, s, tok[u]) : 0;
-                    }
+                    for (int u = 0; u < 4; ++u) info[lane + 32 * u] = nl[u];
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar_i_full(q));
                 }
@@ -490,21 +484,40 @@ ring_paged_weights_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const 
             const int jt = j0 + m * 128;                  // first place of the tile
             const int j = jt + quarter * 32 + lane;       // this thread's place
             float a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
+            uint32_t sr[2][32];
+            // Waits for block `blocks` (+ 1)'s row information and scores and sends for the first 32 columns.
+            auto acquire = [&](uint32_t ahead = 0) {
+                const uint32_t n = blocks + ahead;
+                bool fine = mbar_wait(bar_i_full(n % T::kInfoSlots), (n / T::kInfoSlots) & 1, abort_flag, a.status, kDevPagedSoftmaxS) &&
+                            mbar_wait(bar_s_full(m, n & 1), (n / 2) & 1, abort_flag, a.status, kDevPagedSoftmaxS);
+                fine = __all_sync(0xffffffffu, fine);
+                if (fine) {
+                    tcgen05_fence_after_thread_sync();
+                    tmem_ld_x32(t_s + (n & 1) * 128, sr[0]);
+                }
+                return fine;
+            };
 #pragma unroll 1
             for (int i = 0; i < g.count; ++i, ++blocks) {
                 const int q = blocks % T::kInfoSlots, buf = blocks & 1;
-                ok = mbar_wait(bar_i_full(q), (blocks / T::kInfoSlots) & 1, abort_flag, a.status, kDevPagedSoftmaxS) &&
-                     mbar_wait(bar_s_full(m, buf), (blocks / 2) & 1, abort_flag, a.status, kDevPagedSoftmaxS);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                tcgen05_fence_after_thread_sync();
+                if (i == 0 && !(ok = acquire())) break;
                 const int t0 = (q_first + g.first + i) * a.row_tokens, t1 = min(t0 + a.row_tokens, s.n);
                 const uint32_t info = smem_u32(row_info(q));
                 const bool edge = t0 + a.row_tokens > s.n || jt + 128 > token_hi(a, s, t0) ||
                                   (token_lo(a, s, t1 - 1) > jt && jt + 128 > a.sinks);
-                // 32 columns at a time, the next ones on their way while these are summed
-                uint32_t sr[2][32];
-                tmem_ld_x32(t_s + buf * 128, sr[0]);
+                // The columns whose token sees this place are one interval: behind the first token at or after the place (causal),
+                // before the first whose window has left it.
+                int c0 = 0, c1 = 0;
+                if (edge) {
+                    const int back = j - (s.len - s.n) - t0;  // the place as an index into the tile's tokens
+                    c1 = min(t1 - t0, a.row_tokens);
+                    if (a.causal) c0 = min(max(back, 0), a.row_tokens) * a.group;
+                    if (a.window > 0 && j >= a.sinks)
+                        c1 = static_cast<int>(min(static_cast<int64_t>(c1), max(static_cast<int64_t>(back) + a.window, int64_t(0))));
+                    c1 = j < token_hi(a, s, s.n - 1) ? c1 * a.group : 0;
+                }
+                // 32 columns at a time, the next ones on their way while these are summed (64 at a time: 110 us at the size below, and 114
+                // with the four parts rolled into a loop of two)
 #pragma unroll
                 for (int part = 0; part < 4; ++part) {
                     tmem_wait_ld();
@@ -514,19 +527,14 @@ ring_paged_weights_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const 
                         tcgen05_fence_before_thread_sync();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(bar_s_free(m, buf));
+                        // the next block's waits and first load under this block's last exponentials
+                        if (i + 1 < g.count) ok = acquire(1);
                     }
                     float* sc = reinterpret_cast<float*>(sr[part & 1]);
                     if (edge) {  // scores that do not count become -inf: exp2 of them is 0 whatever they were
 #pragma unroll
-                        for (int v = 0; v < 32; v += 4) {
-                            const uint32_t at = info + 4 * (32 * part + v);
-                            const float4 fh = ld_shared_v4(at + 4 * T::kQRows), fl = ld_shared_v4(at + 8 * T::kQRows);
-                            const int hi[4] = {__float_as_int(fh.x), __float_as_int(fh.y), __float_as_int(fh.z), __float_as_int(fh.w)};
-                            const int lo[4] = {__float_as_int(fl.x), __float_as_int(fl.y), __float_as_int(fl.z), __float_as_int(fl.w)};
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (!(j < hi[e] && (j >= lo[e] || j < a.sinks))) sc[v + e] = -INFINITY;
-                        }
+                        for (int v = 0; v < 32; ++v)
+                            if (32 * part + v < c0 || 32 * part + v >= c1) sc[v] = -INFINITY;
                     }
 #pragma unroll
                     for (int v = 0; v < 32; v += 4) {
@@ -534,12 +542,17 @@ ring_paged_weights_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const 
                         float x0, x1, x2, x3;
                         ffma2(x0, x1, sc[v], sc[v + 1], c, c, nl.x, nl.y);
                         ffma2(x2, x3, sc[v + 2], sc[v + 3], c, c, nl.z, nl.w);
-                        fadd2(a0, a1, a0, a1, ex2_approx(x0), ex2_approx(x1));
+                        if (v % T::kPolyEvery == 0)
+                            ex2_poly2(x0, x1, x0, x1);
+                        else
+                            x0 = ex2_approx(x0), x1 = ex2_approx(x1);
+                        fadd2(a0, a1, a0, a1, x0, x1);
                         fadd2(a2, a3, a2, a3, ex2_approx(x2), ex2_approx(x3));
                     }
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_i_empty(q));
+                if (!ok) break;
             }
             if (!ok) break;
             const float w = (a0 + a1) + (a2 + a3);
