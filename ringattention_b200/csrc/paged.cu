@@ -407,7 +407,7 @@ int ring_paged_attention_fwd(const Ring_paged_params* params) {
     a.unit_rows = plan.unit_rows;
     a.unit_shift = __builtin_ctz(static_cast<unsigned>(plan.unit_rows));
     a.many_tiles = (static_cast<int64_t>(max_new_of(p)) * a.group + plan.unit_rows - 1) / plan.unit_rows > 4;
-    a.start_cost = plan.unit_rows == 256 ? 3 : 2;
+    a.start_cost = plan.unit_rows == 256 ? 4 : 2;
     a.min_blocks = a.start_cost + (plan.unit_rows == 256 ? 2 : 1);
     a.status = plan.unit_rows == 256 ? st->d_status : nullptr;
     cudaStream_t stream = static_cast<cudaStream_t>(p.stream);

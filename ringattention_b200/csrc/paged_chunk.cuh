@@ -36,7 +36,21 @@ enum PagedDeviceStatus : int {
 
 namespace ptx {
 __device__ __forceinline__ void fence_proxy_async_cta() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void bar_sync_all(int threads) { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); }
+// Named barrier that also tells every thread whether any of them brought `pred`.
+__device__ __forceinline__ bool bar_any(int id, int threads, bool pred) {
+    uint32_t any;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %3, 0;\n\t"
+        "barrier.cta.red.or.pred q, %1, %2, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t"
+        "}"
+        : "=r"(any)
+        : "r"(id), "r"(threads), "r"(static_cast<uint32_t>(pred))
+        : "memory");
+    return any != 0;
+}
 }  // namespace ptx
 
 template <class T>
@@ -49,6 +63,9 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     constexpr int kTileBytes = T::kTileBytes;
     constexpr int kBoxBytes = T::kBoxBytes;
     constexpr int kBoxes = T::kBoxesPerTile;
+    // the producers walk the plan too: more registers than in the block kernel, or they spill
+    constexpr int kSoftmaxRegs = 216, kProducerRegs = 72;
+    static_assert(256 * kSoftmaxRegs + 128 * kProducerRegs <= 384 * 168, "what the CTA was launched with");
     constexpr uint32_t kIdescQK = umma_idesc_f16(128, BN, false, false, T::kIsBf16);
     constexpr uint32_t kIdescPV = umma_idesc_f16(128, D, false, true, T::kIsBf16);
 
@@ -103,9 +120,15 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     __syncthreads();
     if (*prior_error != 0) return;  // an earlier launch failed: do nothing (CTA-uniform)
     using U = AttentionUnits<BN>;
-    Share share;
-    Segment g = plan_start<U, T::kNThreads>(a, plan, share, cta, gridDim.x);
-    if (!g.valid) return;  // no share (CTA-uniform)
+    {
+        Share share;
+        const Segment first = plan_start<U, T::kNThreads>(a, plan, share, cta, gridDim.x);
+        if (!first.valid) return;  // no share (CTA-uniform)
+        if (tid == 0) {
+            plan.share = share;
+            plan.seg[0] = first;
+        }
+    }
 
     if (warp == T::kMmaWarp) {
         tmem_alloc(smem_u32(tmem_slot), T::kTmemCols);
@@ -117,6 +140,7 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     const uint32_t tmem_base = *tmem_slot;
 
     // ---- what every role knows of the current segment, and how far its barriers have come
+    Segment g = plan.seg[0];
     SeqView s;
     TileBlocks tb;
     int row0, rows, ntiles, hi_max, lo_min;
@@ -132,29 +156,36 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         hi_max = token_hi(a, s, div_group(a, row0 + rows - 1));
         lo_min = token_lo(a, s, div_group(a, row0));
     };
-    // All threads meet; returns false when the CTA is through (its share is done or a wait ran out).
-    auto end_segment = [&]() {
-        tcgen05_fence_before_thread_sync();
-        bar_sync_all(T::kNThreads);
-        tcgen05_fence_after_thread_sync();
-        if (*abort_flag) return false;
+    auto count_segment = [&]() {
         kv_done += g.count;
         ++segs_done;
         if (ntiles > 1) {
             tile1_done += g.count;
             ++segs1_done;
         }
-        g = plan_next<U>(a, share, g);
+    };
+    // All warps but the loader's, which runs ahead into the next segments, meet; false when the CTA is through (its share is done or
+    // a wait ran out).  Whether one did is decided by the barrier, the same for all: a flag read afterwards might not be.
+    // The S issuer, first to be done with a segment, has left the next one in shared memory (walking the plan in every warp kept
+    // so much alive across the softmax that it spilled).
+    auto end_segment = [&]() {
+        tcgen05_fence_before_thread_sync();
+        const bool gone = bar_any(1, T::kNThreads - 32, *abort_flag != 0);
+        tcgen05_fence_after_thread_sync();
+        if (gone) return false;
+        count_segment();
+        g = plan.seg[segs_done & 1];
         return g.valid != 0;
     };
 
     if (warp >= T::kSoftmaxWarps) {
         // ############################################################## producer warpgroup (warps 8..11)
-        setmaxnreg_dec<T::kProducerRegs>();
+        setmaxnreg_dec<kProducerRegs>();
         if (warp == T::kLoadWarp) {
             // =================================================================== TMA producer: a lane per page
             const int per_block = a.page_shift >= 7 ? 1 : BN >> a.page_shift;  // pages per block (at most 16)
             const int page_rows = min(1 << a.page_shift, BN);                  // places of the block a page holds
+            const Share share = plan.share;
             bool ok = true;
             do {
                 begin_segment();
@@ -194,21 +225,9 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                         __syncwarp();
                     }
                 }
-                if (!ok) {
-                    // given up: wait (bounded) for this warp's copies in flight before shared memory is let go
-#pragma unroll 1
-                    for (int st = 0; st < kStages; ++st) {
-                        const uint32_t nslots = st < T::kKStages ? T::kKStages : T::kVStages;
-                        const uint32_t first = st < T::kKStages ? st : st - T::kKStages;
-                        const uint32_t n = kv_done + g.count;  // fills of this slot are at most those of blocks < n
-                        if (n > first) {
-                            const uint32_t use = (n - 1 - first) / nslots;
-                            for (int spin = 0; spin < 20000 && !mbar_test_wait(bar_kv_full(st), use & 1) && !mbar_test_wait(bar_kv_full(st), (use + 1) & 1); ++spin) {
-                            }
-                        }
-                    }
-                }
-            } while (end_segment());
+            count_segment();
+                g = plan_next<U>(a, share, g);
+            } while (ok && g.valid);
         } else if (warp == T::kMmaWarp) {
             // =================================================================== UMMA issuer: S = Q K^T, both tiles
             uint32_t products = 0;  // S products issued so far; number n - 1 must have been read out before number n
@@ -239,6 +258,7 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                             ++products;
                         }
                     }
+                    plan.seg[(segs_done + 1) & 1] = plan_next<U>(a, plan.share, g);
                 }
                 __syncwarp();
             } while (end_segment());
@@ -263,14 +283,16 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                     // V rows that no row of the unit sees: zeros (both issuers may write them, the same values)
                     const int j0 = tb.block(g.first + i) * BN;
                     if (j0 + BN > hi_max || (j0 < lo_min && j0 + BN > a.sinks)) {
+                        const uint32_t to = smem_kv(vslot) + (lane & 7) * 16;
+                        auto clear = [&](int r, int end) {  // rows [r, end): four rows of one box at a time
 #pragma unroll 1
-                        for (int r = 0; r < BN; ++r) {
-                            const int j = j0 + r;
-                            if (j >= hi_max || (j < lo_min && j >= a.sinks)) {
-                                if (lane < kBoxes * 8)
-                                    st_shared_v4(smem_kv(vslot) + (lane >> 3) * kBoxBytes + r * 128 + (lane & 7) * 16, 0u, 0u, 0u, 0u);
+                            for (r += lane >> 3; r < end; r += 4) {
+#pragma unroll
+                                for (int bx = 0; bx < kBoxes; ++bx) st_shared_v4(to + bx * kBoxBytes + r * 128, 0u, 0u, 0u, 0u);
                             }
-                        }
+                        };
+                        clear(max(hi_max - j0, 0), BN);
+                        clear(max(a.sinks - j0, 0), min(lo_min - j0, BN));
                         fence_proxy_async_cta();
                         __syncwarp();
                     }
@@ -294,7 +316,7 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         }
     } else {
         // ############################################################## softmax warpgroups (warps 0..7)
-        setmaxnreg_inc<T::kSoftmaxRegs>();
+        setmaxnreg_inc<kSoftmaxRegs>();
         const int t = warp >> 2;
         const int quarter = warp & 3;
         const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
@@ -317,12 +339,10 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
 #pragma unroll
                     for (int u = 0; u < 32 / kRowsPer; ++u) {
                         const int r = warp_row + u * kRowsPer + lane / kChunks;
-                        val[u] = make_uint4(0u, 0u, 0u, 0u);
-                        if (r < rows) {
-                            const int at = row0 + r, tok = div_group(a, at);
-                            val[u] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + static_cast<int64_t>(s.q0 + tok) * a.q_token +
-                                                                     static_cast<int64_t>(g.h * a.group + (at - tok * a.group)) * a.q_head + ch * 8);
-                        }
+                        // the last row again instead of a row behind it: a branch around the load would take the loads one by one
+                        const int at = row0 + min(r, rows - 1), tok = div_group(a, at);
+                        val[u] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + static_cast<int64_t>(s.q0 + tok) * a.q_token +
+                                                                 static_cast<int64_t>(g.h * a.group + (at - tok * a.group)) * a.q_head + ch * 8);
                     }
 #pragma unroll
                     for (int u = 0; u < 32 / kRowsPer; ++u) {
@@ -339,10 +359,12 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                 const int hi = token_hi(a, s, tok), lo = token_lo(a, s, tok);
                 const int tile_first = div_group(a, row0 + t * 128), tile_last = div_group(a, row0 + min(t * 128 + 127, rows - 1));
                 const int hi_min = token_hi(a, s, tile_first), lo_max = token_lo(a, s, tile_last);
-                auto pages_of = [&](int i) {  // which pages of block i exist, a bit each
+                auto pages_of = [&](int i) {  // which pages of block i exist or lie behind every row's limit, a bit each
                     int have = 0;
-                    if (lane < per_block && i < g.count)
-                        have = page_of(a, g.b, (tb.block(g.first + i) * BN >> a.page_shift) + lane) >= 0;
+                    if (lane < per_block && i < g.count) {
+                        const int pg = (tb.block(g.first + i) * BN >> a.page_shift) + lane;
+                        have = (static_cast<int64_t>(pg) << a.page_shift) >= hi_max || page_of(a, g.b, pg) >= 0;
+                    }
                     return have;
                 };
                 int have_next = pages_of(0);
@@ -508,7 +530,7 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                         else
                             a.lse[static_cast<int64_t>(s.q0 + tok) * a.heads + g.h * a.group + (row0 + row - tok * a.group)] = lse;
                     }
-                    if (slot == 2 * cta + 1 && tid == 0) note_cut(a, share, g, cta, row0, rows, s.q0);
+                    if (slot == 2 * cta + 1 && tid == 0) note_cut(a, plan.share, g, cta, row0, rows, s.q0);
                 }
             }
         } while (end_segment());

@@ -210,6 +210,35 @@ __device__ __forceinline__ void cut_unit(const PagedArgs& a, Segment& g, int64_t
     g.valid = g.count > 0;
 }
 
+// The segment after `g` in the share.  Every thread that needs it works it out.
+template <class U>
+__device__ __forceinline__ Segment plan_next(const PagedArgs& a, const Share& sh, Segment g) {
+    const int64_t at = g.begin + a.start_cost + g.unit_blocks;  // where the next unit begins
+    g.valid = 0;
+    if (g.first + g.count < g.unit_blocks || at >= sh.x1) return g;
+    SeqView s;
+    if (g.tile + 1 < g.tiles) {
+        ++g.tile;
+        s = seq_view(a, g.b);
+    } else if (g.h + 1 < a.kv_heads) {
+        ++g.h;
+        g.tile = 0;
+        s = seq_view(a, g.b);
+    } else {
+        g.h = 0;
+        g.tile = 0;
+        do {
+            if (++g.b >= a.batch) return g;
+            s = seq_view(a, g.b);
+            g.tiles = U::tiles(a, s);
+        } while (g.tiles == 0);
+    }
+    g.begin = at;
+    g.unit_blocks = U::blocks(a, s, g.tile);
+    cut_unit(a, g, at, sh.x1);
+    return g;
+}
+
 // The first segment of the share: x0 lies in sequence b, whose list begins at `before` and costs `own` per head.  Called by a
 // whole warp, which gets the result in every lane.
 template <class U>
@@ -254,6 +283,9 @@ struct PlanShared {
     int64_t warp_sum[32];
     int found_b;
     int64_t found_before, found_own;
+    // for kernels whose warps have no registers to spare for them: the share, and the current and the next segment
+    Share share;
+    Segment seg[2];
 };
 
 // This CTA's share and its first segment (all threads call it and get the same; `p` is scratch).
@@ -341,35 +373,6 @@ __device__ __forceinline__ Segment plan_start(const PagedArgs& a, PlanShared& p,
     }
     __syncthreads();
     return first_segment<U>(a, sh, p.found_b, p.found_before, p.found_own);
-}
-
-// The segment after `g` in the share.  Every thread that needs it works it out.
-template <class U>
-__device__ __forceinline__ Segment plan_next(const PagedArgs& a, const Share& sh, Segment g) {
-    const int64_t at = g.begin + a.start_cost + g.unit_blocks;  // where the next unit begins
-    g.valid = 0;
-    if (g.first + g.count < g.unit_blocks || at >= sh.x1) return g;
-    SeqView s;
-    if (g.tile + 1 < g.tiles) {
-        ++g.tile;
-        s = seq_view(a, g.b);
-    } else if (g.h + 1 < a.kv_heads) {
-        ++g.h;
-        g.tile = 0;
-        s = seq_view(a, g.b);
-    } else {
-        g.h = 0;
-        g.tile = 0;
-        do {
-            if (++g.b >= a.batch) return g;
-            s = seq_view(a, g.b);
-            g.tiles = U::tiles(a, s);
-        } while (g.tiles == 0);
-    }
-    g.begin = at;
-    g.unit_blocks = U::blocks(a, s, g.tile);
-    cut_unit(a, g, at, sh.x1);
-    return g;
 }
 
 // Where a segment's result goes: -1 = the unit is whole, straight to the output; else its partial slot.
