@@ -235,11 +235,11 @@ int cache_map(CUtensorMap* tm, const ring::PagedArgs& a, const void* base, int64
     return RING_OK;
 }
 
-template <int D, bool kBf16>
+template <int D, bool kBf16, bool kWindow>
 int launch_chunk(const ring::PagedArgs& a, const AttentionPlan& plan, DeviceState* st, cudaStream_t stream) {
     using T = Ring_fwd_traits<D, 256, 128, 12, typename std::conditional<kBf16, __nv_bfloat16, __half>::type>;
-    auto kernel = &ring::ring_paged_chunk_kernel<T>;
-    int rc = set_smem(kernel, T::kSmemSize, &st->paged_attr_set[8 + (D == 128) * 2 + kBf16]);
+    auto kernel = &ring::ring_paged_chunk_kernel<T, kWindow>;
+    int rc = set_smem(kernel, T::kSmemSize, &st->paged_attr_set[8 + kWindow * 20 + (D == 128) * 2 + kBf16]);
     if (rc) return rc;
     CUtensorMap tk, tv;
     if ((rc = cache_map(&tk, a, a.k, a.k_page, a.k_head, a.k_place, D, kBf16))) return rc;
@@ -250,7 +250,8 @@ int launch_chunk(const ring::PagedArgs& a, const AttentionPlan& plan, DeviceStat
 
 template <int D, bool kBf16>
 int launch_attention(const ring::PagedArgs& a, const AttentionPlan& plan, DeviceState* st, cudaStream_t stream) {
-    if (plan.unit_rows == 256) return launch_chunk<D, kBf16>(a, plan, st, stream);
+    if (plan.unit_rows == 256)
+        return a.window > 0 ? launch_chunk<D, kBf16, true>(a, plan, st, stream) : launch_chunk<D, kBf16, false>(a, plan, st, stream);
     if (plan.unit_rows == 16) return launch_rows<D, kBf16, 1>(a, plan, st, stream);
     return launch_rows<D, kBf16, 2>(a, plan, st, stream);
 }

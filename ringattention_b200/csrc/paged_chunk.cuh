@@ -53,9 +53,39 @@ __device__ __forceinline__ bool bar_any(int id, int threads, bool pred) {
 }
 }  // namespace ptx
 
-template <class T>
+// A window's edge, or a page that does not exist: the scores of block col0 that nobody may see are overwritten where they are, in TMEM,
+// 32 columns at a time.  By a warp; lo is the thread's row's lower limit.  A call, so that its registers are not the main loop's:
+// as one more mask on the 128 scores in registers it cost every block 8 %.
+template <bool kWindow>
+__device__ __noinline__ void hide_scores(const PagedArgs& a, uint32_t t_s, int b, int col0, int lo) {
+    using namespace ptx;
+    const int lane = threadIdx.x & 31;
+    const int per_block = a.page_shift >= 7 ? 1 : 128 >> a.page_shift;
+    const uint32_t have = __ballot_sync(0xffffffffu, lane < per_block && page_of(a, b, (col0 >> a.page_shift) + lane) >= 0);
+#pragma unroll 1
+    for (int w = 0; w < 128; w += 32) {
+        // 32 columns a word: all without [sink, from), and only in pages that exist
+        auto below = [&](int n) { return n <= w ? 0u : (n >= w + 32 ? 0xffffffffu : (1u << (n - w)) - 1u); };
+        uint32_t see = kWindow ? below(a.sinks - col0) | ~below(lo - col0) : 0xffffffffu;
+#pragma unroll 1
+        for (int v = 0; v < 32; v += 8)
+            if (!((have >> ((w + v) >> min(a.page_shift, 7))) & 1u)) see &= ~(0xffu << v);
+        uint32_t x[32];
+        tmem_ld_x32(t_s + w, x);
+        tmem_wait_ld();
+#pragma unroll
+        for (int v = 0; v < 32; ++v)
+            if (!((see >> v) & 1u)) x[v] = 0xff800000u;  // -inf
+        tmem_st_x32(t_s + w, x);
+    }
+    tmem_wait_st();
+}
+
+// kWindow: the call has a window (its limits held across the main loop cost every block 8 %).
+template <class T, bool kWindow>
 __global__ void __launch_bounds__(T::kNThreads, 1)
-ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const PagedArgs a) {
+ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                        const __grid_constant__ PagedArgs a) {
     using namespace ptx;
     constexpr int D = T::kHeadDim;
     constexpr int BN = T::kBlockN;
@@ -78,6 +108,10 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + T::kNumBarriers);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* prior_error = reinterpret_cast<volatile int*>(tmem_slot + 2);
+    // Block n & 7: a page of it that somebody sees does not exist.  The loader is less than eight blocks ahead of the softmax (a V
+    // slot is free only when its block's product is done), and its store is ordered before the block's scores by the barriers between.
+    volatile int* gap = reinterpret_cast<volatile int*>(tmem_slot + 3);
+    static_assert(T::kNumBarriers * 8 + 12 + 32 <= 256 && T::kVStages < 7, "tail of shared memory, depth of the V ring");
 
     const uint32_t bar0 = smem_u32(bars);
     auto bar_q_full = [&](int t) { return bar0 + 8u * t; };
@@ -193,13 +227,13 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                     if (lane >= per_block || i >= g.count) return a.num_pages;
                     const int j0 = tb.block(g.first + i) * BN + lane * page_rows;
                     if (j0 >= hi_max || (j0 + page_rows <= lo_min && j0 >= a.sinks)) return a.num_pages;
-                    const int id = page_of(a, g.b, j0 >> a.page_shift);
-                    return id < 0 ? a.num_pages : id;
+                    return page_of(a, g.b, j0 >> a.page_shift);  // -1: there is none
                 };
                 int id = page_id(0);
 #pragma unroll 1
                 for (int i = 0; i < g.count && ok; ++i) {
-                    const int id_now = id;
+                    const bool missing = __any_sync(0xffffffffu, id < 0);
+                    const int id_now = id < 0 ? a.num_pages : id;
                     id = page_id(i + 1);
                     const int in_page = (tb.block(g.first + i) * BN) & ((1 << a.page_shift) - 1) & ~(BN - 1);
                     const uint32_t n = kv_done + i;
@@ -213,7 +247,10 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                             ok = __all_sync(0xffffffffu, ok);
                             if (!ok) break;
                         }
-                        if (lane == 0) mbar_arrive_expect_tx(bar_kv_full(slot), kTileBytes);
+                        if (lane == 0) {
+                            if (kv == 0) gap[n & 7] = missing;
+                            mbar_arrive_expect_tx(bar_kv_full(slot), kTileBytes);
+                        }
                         __syncwarp();
                         if (lane < per_block) {
                             const CUtensorMap* tm = kv == 0 ? &tm_k : &tm_v;
@@ -324,8 +361,6 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         const uint32_t t_p = tmem_base + lane_addr + T::kTmemP0 + t * T::kTmemPCols;
         const uint32_t t_o = tmem_base + lane_addr + T::kTmemO0 + t * D;
         const float c = a.scale_log2;
-        const int per_block = a.page_shift >= 7 ? 1 : BN >> a.page_shift;
-        const uint32_t all_pages = (1u << per_block) - 1u;
         do {
             begin_segment();
             if (t < ntiles) {
@@ -356,33 +391,25 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                 // ---- limits of this thread's row, and of the tile (for the blocks that need no mask)
                 const int row = warp_row + lane;
                 const int tok = div_group(a, row0 + min(row, rows - 1));
-                const int hi = token_hi(a, s, tok), lo = token_lo(a, s, tok);
+                const int hi = token_hi(a, s, tok), lo = kWindow ? token_lo(a, s, tok) : 0;
                 const int tile_first = div_group(a, row0 + t * 128), tile_last = div_group(a, row0 + min(t * 128 + 127, rows - 1));
-                const int hi_min = token_hi(a, s, tile_first), lo_max = token_lo(a, s, tile_last);
-                auto pages_of = [&](int i) {  // which pages of block i exist or lie behind every row's limit, a bit each
-                    int have = 0;
-                    if (lane < per_block && i < g.count) {
-                        const int pg = (tb.block(g.first + i) * BN >> a.page_shift) + lane;
-                        have = (static_cast<int64_t>(pg) << a.page_shift) >= hi_max || page_of(a, g.b, pg) >= 0;
-                    }
-                    return have;
-                };
-                int have_next = pages_of(0);
-
+                const int hi_min = token_hi(a, s, tile_first), lo_max = kWindow ? token_lo(a, s, tile_last) : 0;
                 float m_run = -INFINITY;
                 float l_run = 0.f;
                 bool ok = true;
 #pragma unroll 1
                 for (int i = 0; i < g.count; ++i) {
                     const uint32_t n = (t ? tile1_done : kv_done) + i;
-                    const uint32_t have = __ballot_sync(0xffffffffu, have_next);
-                    have_next = pages_of(i + 1);
                     uint32_t sr[128];
                     float* sc = reinterpret_cast<float*>(sr);
                     ok = mbar_wait(bar_s_full(t), n & 1, abort_flag, a.status, kDevPagedSoftmaxS);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tcgen05_fence_after_thread_sync();
+                    const int col0 = tb.block(g.first + i) * BN;
+                    if ((kWindow && lo_max > col0 && col0 + BN > a.sinks) || gap[(kv_done + i) & 7]) {
+                        hide_scores<kWindow>(a, t_s, g.b, col0, lo);
+                    }
 #pragma unroll
                     for (int u = 0; u < 4; ++u) tmem_ld_x32(t_s + 32 * u, *reinterpret_cast<uint32_t(*)[32]>(&sr[32 * u]));
                     tmem_wait_ld();
@@ -390,16 +417,7 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar_s_free);
 
-                    const int col0 = tb.block(g.first + i) * BN;
-                    const bool hidden = lo_max > col0 && col0 + BN > a.sinks;
-                    if (hidden || have != all_pages) {
-                        const int limit = hi - col0, from = lo - col0, sink = a.sinks - col0;
-#pragma unroll
-                        for (int u = 0; u < 128; ++u) {
-                            const bool see = u < limit && (u >= from || u < sink) && ((have >> (u >> a.page_shift)) & 1u);
-                            if (!see) sc[u] = -INFINITY;
-                        }
-                    } else if (col0 + BN > hi_min) {
+                    if (col0 + BN > hi_min) {
                         const int limit = hi - col0;
 #pragma unroll
                         for (int u = 0; u < 128; ++u)
