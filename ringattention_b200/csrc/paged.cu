@@ -211,7 +211,7 @@ int launch_rows(const ring::PagedArgs& a, const AttentionPlan& plan, DeviceState
     int rc = set_smem(kernel, T::kSmem, &st->paged_attr_set[(MT - 1) * 4 + (D == 128) * 2 + kBf16]);
     if (rc) return rc;
     if ((rc = launch(kernel, dim3(plan.grid), dim3(T::kThreads), T::kSmem, stream, a))) return rc;
-    return launch(&ring::ring_paged_join_kernel<D, kBf16, 4>, dim3(plan.grid, plan.rows), dim3(128), 0, stream, a, plan.unit_rows);
+    return launch(&ring::ring_paged_join_kernel<D, kBf16, 4>, dim3(plan.grid, plan.rows < 8 ? plan.rows : 8), dim3(128), 0, stream, a, plan.unit_rows);
 }
 
 // The cache as a 4-D map [pages, kv_heads, page_size, dim]: a box is 64 columns of min(page_size, 128) places of one page and head,
@@ -245,7 +245,7 @@ int launch_chunk(const ring::PagedArgs& a, const AttentionPlan& plan, DeviceStat
     if ((rc = cache_map(&tk, a, a.k, a.k_page, a.k_head, a.k_place, D, kBf16))) return rc;
     if ((rc = cache_map(&tv, a, a.v, a.v_page, a.v_head, a.v_place, D, kBf16))) return rc;
     if ((rc = launch(kernel, dim3(plan.grid), dim3(T::kNThreads), T::kSmemSize, stream, tk, tv, a))) return rc;
-    return launch(&ring::ring_paged_join_kernel<D, kBf16, 1>, dim3(plan.grid, 32), dim3(128), 0, stream, a, plan.unit_rows);
+    return launch(&ring::ring_paged_join_kernel<D, kBf16, 1>, dim3(plan.grid, 16), dim3(128), 0, stream, a, plan.unit_rows);
 }
 
 template <int D, bool kBf16>

@@ -417,39 +417,95 @@ __global__ void __launch_bounds__(T::kThreads) ring_paged_rows_kernel(const Page
     }
 }
 
-// Joins the partials of the units that share boundaries have cut: CTA (c, y) takes rows y, y + gridDim.y, ... of the unit that
-// begins in share c.  out = sum_p exp(lse_p - lse) out_p with lse over all partials first, so that the loads of the
-// second pass do not wait on one another.  kSplit warps share the partials of one row.  Bound by latency.
+// Joins the partials of the units that share boundaries have cut: CTA (c, y) takes rows of the unit that begins in share c.
+// out = sum_p exp(lse_p - lse) out_p with lse over all partials first, so that no load waits on another one's value.
+// Bound by latency, so everything that can be in flight is: units of few partials take four rows a warp with all their loads at
+// once; others (long sequences: tens of shares a unit) give the partials of one row to kSplit warps.
 template <int D, bool kBf16, int kSplit>
-__global__ void __launch_bounds__(128) ring_paged_join_kernel(const PagedArgs a, int unit_rows) {
+__global__ void __launch_bounds__(32 * (kSplit > 4 ? kSplit : 4)) ring_paged_join_kernel(const PagedArgs a, int unit_rows) {
     using namespace ptx;
-    __shared__ float4 sm_o[4][32];
+    constexpr int kWarps = kSplit > 4 ? kSplit : 4;
+    __shared__ float4 sm_o[kWarps][32];
     griddep_wait();
-    if (a.status && *reinterpret_cast<volatile int*>(a.status) != 0) return;  // a wait ran out: the partials are not whole
     const int c = blockIdx.x;
-    const int4 more = a.cut[2 * c + 1];
+    const int4 u = a.cut[2 * c], more = a.cut[2 * c + 1];
+    if (a.status && *reinterpret_cast<volatile int*>(a.status) != 0) return;  // a wait ran out: the partials are not whole
     const int parts = more.x;
     if (parts <= 1) return;
-    const int4 u = a.cut[2 * c];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int kLanes = D / 4;          // lanes per row
-    constexpr int kSub = 32 / kLanes;      // partials a warp reads at once
-    constexpr int kRowsAtOnce = 4 / kSplit;
-    constexpr int kPieces = kSplit * kSub;
+    constexpr int kSub = 32 / kLanes;      // rows, or partials of one, a warp reads at once
     const int sub = lane / kLanes, col = (lane % kLanes) * 4;
+    auto at = [&](int p, int row) { return static_cast<int64_t>(p == 0 ? 2 * c + 1 : 2 * (c + p)) * unit_rows + row; };
+    auto put = [&](int row, const float4& v, float lse) {
+        const int r = u.z + row, tok = div_group(a, r);
+        const int64_t token = more.y + tok;
+        const int head = u.y * a.group + (r - tok * a.group);
+        const int64_t to = token * a.out_token + head * a.out_head + col;
+        if (a.out_fp32)
+            *reinterpret_cast<float4*>(static_cast<float*>(a.out) + to) = v;
+        else
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + to) = make_uint2(pack16<kBf16>(v.x, v.y), pack16<kBf16>(v.z, v.w));
+        if (col == 0) a.lse[token * a.heads + head] = lse;
+    };
+    auto add = [](float4& acc, const float4& v, float w) {
+        acc.x = fmaf(v.x, w, acc.x);
+        acc.y = fmaf(v.y, w, acc.y);
+        acc.z = fmaf(v.z, w, acc.z);
+        acc.w = fmaf(v.w, w, acc.w);
+    };
+    if (parts <= 4) {
+        constexpr int kR = 4;  // rows of a lane
+        for (int r0 = (blockIdx.y * kWarps + warp) * kR * kSub; r0 < u.w; r0 += gridDim.y * kWarps * kR * kSub) {
+            float e[kR][4];
+            float4 v[kR][4];
+#pragma unroll
+            for (int k = 0; k < kR; ++k) {
+                const int row = min(r0 + k * kSub + sub, u.w - 1);
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    e[k][p] = -INFINITY;
+                    v[k][p] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (p < parts) {  // the same for all threads
+                        e[k][p] = a.part_lse[at(p, row)];
+                        v[k][p] = *reinterpret_cast<const float4*>(a.part_o + at(p, row) * D + col);
+                    }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kR; ++k) {
+                const int row = r0 + k * kSub + sub;
+                const float mx = fmaxf(fmaxf(e[k][0], e[k][1]), fmaxf(e[k][2], e[k][3]));
+                float l = 0.f;
+#pragma unroll
+                for (int p = 0; p < 4; ++p) l += e[k][p] == -INFINITY ? 0.f : expf(e[k][p] - mx);
+                const float lse = (l > 0.f || l != l) ? (mx == -INFINITY ? 0.f : mx) + logf(l) : -INFINITY;
+                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int p = 0; p < 4; ++p) add(acc, v[k][p], e[k][p] == -INFINITY ? 0.f : expf(e[k][p] - lse));
+                if (row < u.w) put(row, acc, lse);
+            }
+        }
+        return;
+    }
+    constexpr int kRowsAtOnce = kWarps / kSplit;
+    constexpr int kPieces = kSplit * kSub;
     const int piece = (warp % kSplit) * kSub + sub;
     for (int r0 = blockIdx.y * kRowsAtOnce; r0 < u.w; r0 += gridDim.y * kRowsAtOnce) {
         const int row = r0 + warp / kSplit;
         const bool live = row < u.w;
-        auto at = [&](int p) { return static_cast<int64_t>(p == 0 ? 2 * c + 1 : 2 * (c + p)) * unit_rows + row; };
         float lse = -INFINITY;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         if (live) {
             float mx = -INFINITY, l = 0.f;
-            for (int p = lane; p < parts; p += 32) {
-                const float e = a.part_lse[at(p)];
-                const float m2 = fmaxf(mx, e);
-                l = (mx == m2 ? l : l * expf(mx - m2)) + (e == -INFINITY ? 0.f : expf(e - m2));
+            for (int p0 = lane; p0 < parts; p0 += 128) {
+                float e[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) e[k] = p0 + 32 * k < parts ? a.part_lse[at(p0 + 32 * k, row)] : -INFINITY;
+                const float m2 = fmaxf(fmaxf(fmaxf(mx, e[0]), fmaxf(e[1], e[2])), e[3]);
+                l = mx == m2 ? l : l * expf(mx - m2);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) l += e[k] == -INFINITY ? 0.f : expf(e[k] - m2);
                 mx = m2;
             }
 #pragma unroll
@@ -462,41 +518,20 @@ __global__ void __launch_bounds__(128) ring_paged_join_kernel(const PagedArgs a,
             if (l > 0.f || l != l) lse = (mx == -INFINITY ? 0.f : mx) + logf(l);
 #pragma unroll 8
             for (int p = piece; p < parts; p += kPieces) {
-                const float e = a.part_lse[at(p)];
-                const float w = e == -INFINITY ? 0.f : expf(e - lse);
-                const float4 v = *reinterpret_cast<const float4*>(a.part_o + at(p) * D + col);
-                acc.x = fmaf(v.x, w, acc.x);
-                acc.y = fmaf(v.y, w, acc.y);
-                acc.z = fmaf(v.z, w, acc.z);
-                acc.w = fmaf(v.w, w, acc.w);
+                const float e = a.part_lse[at(p, row)];
+                const float4 v = *reinterpret_cast<const float4*>(a.part_o + at(p, row) * D + col);
+                add(acc, v, e == -INFINITY ? 0.f : expf(e - lse));
             }
         }
         if (kPieces > 1) {
             sm_o[warp][lane] = acc;
             __syncthreads();
             if (live && piece == 0) {
-                for (int p = 1; p < kPieces; ++p) {
-                    const float4 v = sm_o[warp + p / kSub][(p % kSub) * kLanes + lane];
-                    acc.x += v.x;
-                    acc.y += v.y;
-                    acc.z += v.z;
-                    acc.w += v.w;
-                }
+                for (int p = 1; p < kPieces; ++p) add(acc, sm_o[warp + p / kSub][(p % kSub) * kLanes + lane], 1.f);
             }
             __syncthreads();
         }
-        if (live && piece == 0) {
-            const int r = u.z + row, tok = div_group(a, r);
-            const int64_t token = more.y + tok;
-            const int head = u.y * a.group + (r - tok * a.group);
-            const int64_t to = token * a.out_token + head * a.out_head + col;
-            if (a.out_fp32)
-                *reinterpret_cast<float4*>(static_cast<float*>(a.out) + to) = acc;
-            else
-                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + to) =
-                    make_uint2(pack16<kBf16>(acc.x, acc.y), pack16<kBf16>(acc.z, acc.w));
-            if (col == 0) a.lse[token * a.heads + head] = lse;
-        }
+        if (live && piece == 0) put(row, acc, lse);
     }
 }
 
