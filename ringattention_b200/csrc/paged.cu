@@ -192,10 +192,15 @@ struct AttentionPlan {
 
 int64_t round256(int64_t x) { return (x + 255) / 256 * 256; }
 
+// Which kernel, by the query rows per K/V head (new tokens x group).  Microseconds for 16 sequences of 8192 places, 8 K/V heads,
+// bf16, pages of 64 (16-row units / 32-row units of the few-rows kernel / the 256-row tcgen05 kernel):
+//   D = 128   16 rows 101 / 123 / 104    24 rows 179 / 128 / 106    32 rows 181 / 131 / 107    64 rows 340 / 248 / 110
+//   D = 64    16 rows  53 /  56 /  99    24 rows  75 /  58 / 100    32 rows  76 /  59 / 100    64 rows 173 / 100 / 100
+// At D = 128 the 32-row units spill, so there the tcgen05 kernel takes over at 17 rows, at D = 64 at 33.
 AttentionPlan attention_plan(const Ring_paged_params& p, int sm_count) {
     AttentionPlan r;
     const int64_t rows = static_cast<int64_t>(max_new_of(p)) * (p.heads / p.kv_heads);
-    r.unit_rows = rows <= 16 ? 16 : (rows <= 32 ? 32 : 256);
+    r.unit_rows = rows <= 16 ? 16 : (rows <= 32 && p.dim == 64 ? 32 : 256);
     r.rows = static_cast<int>(rows < 1 ? 1 : (rows < r.unit_rows ? rows : r.unit_rows));
     r.grid = r.unit_rows <= 32 ? 2 * sm_count : sm_count;  // two CTAs of the few-rows kernel fit an SM, one of the other
     r.o_bytes = round256(int64_t(2) * r.grid * r.unit_rows * p.dim * 4);
@@ -252,8 +257,10 @@ template <int D, bool kBf16>
 int launch_attention(const ring::PagedArgs& a, const AttentionPlan& plan, DeviceState* st, cudaStream_t stream) {
     if (plan.unit_rows == 256)
         return a.window > 0 ? launch_chunk<D, kBf16, true>(a, plan, st, stream) : launch_chunk<D, kBf16, false>(a, plan, st, stream);
-    if (plan.unit_rows == 16) return launch_rows<D, kBf16, 1>(a, plan, st, stream);
-    return launch_rows<D, kBf16, 2>(a, plan, st, stream);
+    if constexpr (D == 64) {
+        if (plan.unit_rows == 32) return launch_rows<D, kBf16, 2>(a, plan, st, stream);
+    }
+    return launch_rows<D, kBf16, 1>(a, plan, st, stream);
 }
 
 // ---- weights -------------------------------------------------------------------------------------------------------
@@ -265,6 +272,9 @@ struct WeightsPlan {
     int64_t bytes() const { return part_bytes + cut_bytes; }
 };
 
+// Which form, by the query rows per K/V head.  Microseconds for 16 sequences of 8192 places, 8 K/V heads, D = 128, bf16 (rows form
+// holding 8 rows / 32 rows in registers, chunk form): 8 rows 59 / 76 / 133, 16 rows 99 / 76 / 134, 32 rows 155 / 78 / 134,
+// 40 rows 184 / 189 / 140, 64 rows 276 / 214 / 135.
 WeightsPlan weights_plan(const Ring_paged_params& p, int sm_count) {
     WeightsPlan r;
     const int64_t group = p.heads / p.kv_heads, rows = max_new_of(p) * group;
@@ -408,6 +418,8 @@ int ring_paged_attention_fwd(const Ring_paged_params* params) {
     a.unit_rows = plan.unit_rows;
     a.unit_shift = __builtin_ctz(static_cast<unsigned>(plan.unit_rows));
     a.many_tiles = (static_cast<int64_t>(max_new_of(p)) * a.group + plan.unit_rows - 1) / plan.unit_rows > 4;
+    // in blocks: about 7 thousand clocks of lookups, first loads and write-out against 3 thousand a block of 256 rows, and 3 thousand
+    // against 1.4 thousand of the few-rows kernel
     a.start_cost = plan.unit_rows == 256 ? 4 : 2;
     a.min_blocks = a.start_cost + (plan.unit_rows == 256 ? 2 : 1);
     a.status = plan.unit_rows == 256 ? st->d_status : nullptr;

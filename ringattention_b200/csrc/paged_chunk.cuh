@@ -9,7 +9,13 @@
 //     warp; pages that nobody sees are fetched from behind the last page, which reads as zeros without traffic;
 //   * V rows that no row of the unit sees are zeroed in shared memory on the blocks at the edges (0 x NaN is not 0);
 //   * a CTA walks an equal share of all units' blocks (paged_plan.cuh), with running phase counters across units; a unit that a
-//     share boundary cuts leaves normalised fp32 partials.
+//     share boundary cuts leaves normalised fp32 partials; the loader warp runs ahead into the next unit.
+// P is rounded to the inputs' type as in the block kernel (at most 2^-8 of it for bf16, 2^-11 for fp16); sums and statistics are fp32.
+//
+// Measured: 2048 tokens over 32768 places, 32 / 8 heads, D = 128, bf16: 1.04 ms in a steady loop (1.03 PFLOP/s, 0.61 of the measured
+// cuBLAS burst rate; 0.87 ms, 1.22 PFLOP/s from idle), about 3 thousand clocks a block of 2 x 128 rows by 128 places as in the block kernel,
+// bound by its S-buffer chain.  4 chunks of 130-515 tokens over 1500-6001 places, 16 heads: 114 us; a quarter of its rows are
+// padding of the last tiles and joining the cut units takes 14 us.
 #pragma once
 
 #include <cstdint>

@@ -6,8 +6,13 @@
 // barrier.  S = Q K^T and O += P V are mma.sync m16n8k16: the arithmetic (4 D per row and place, rows padded to
 // 16) is a small part of what the legacy tensor path does in the time the places take from HBM, and its 16-row tile
 // fits these row counts where a 128-row tcgen05 tile would be mostly padding.  Running maximum, sum and O stay in registers (fp32);
-// P is rounded to the inputs' type for the product (relative half step 2^-9 bf16, 2^-12 fp16, random in sign; the sum l uses
-// the unrounded values).  The warps' partials are joined in shared memory at the end of a unit.
+// P is rounded to the inputs' type for the product (by at most 2^-8 of it for bf16, 2^-11 for fp16; the sum l takes the
+// unrounded values).  The warps' partials are joined in shared memory at the end of a unit.
+//
+// Measured: 30 sequences of 300 to 8192 places, 8 K/V heads, group 4, D = 128, bf16, pages of 16: 93 us, 5.9 TB/s, 0.90 of the
+// measured copy rate; 2 x 131072 places, 2 K/V heads, group 8: 47 us of reading (5.7 TB/s) + 8 us of joining 74 partials a unit.  Two
+// CTAs of four warps an SM, three stages of 8 KiB a warp: 128 KiB on their way per SM.  Page ids
+// come 32 groups of 8 places at a time, one batch ahead: loaded step by step they put a second latency before every unit's first rows.
 #pragma once
 
 #include <cstdint>

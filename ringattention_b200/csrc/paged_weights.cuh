@@ -6,8 +6,12 @@
 // places are the M side of mma.sync m16n8k16 and the query rows the N side, so 8 rows cost one instruction per 16 places.
 //
 // Chunk form (many rows): two 128 x 128 x D products per 128 query rows and 256 places, then 32768 exponentials and their sums.  The
-// MUFU does 16 exponentials a clock: 2048 clocks against 1024 of tensor time at D = 128, so the exponentials bound it.  S^T = K Q^T with the places as TMEM lanes: a softmax-free epilogue
-// thread owns one place, its sum over the columns stays in a register, and nothing crosses threads.
+// MUFU does 16 exponentials a clock: 2048 clocks against 1024 of tensor time at D = 128, so the exponentials bound it.  S^T = K Q^T
+// with the places as TMEM lanes: a thread owns one place, its sum over the columns stays in a register, nothing crosses threads.
+//
+// Measured: rows form, 16 sequences of 500 to 8192 places, 8 K/V heads, group 4, D = 128, one token: 37 us, 4.1 TB/s (launch, plan and the
+// last steps are a third of it).  Chunk form, 1024 tokens over 8192 places, 32 / 8 heads, D = 128: 102 us, about 2500 clocks a block
+// against the 2048 of the exponentials; moving a quarter of them to the FMA pipe: 105 -> 102 us, half: 107.
 #pragma once
 
 #include <cstdint>
