@@ -262,8 +262,8 @@ int ring_static_status(int* status_out, void* stream);
  * power of two >= 8.
  * Sequences.  page_table[b * table_stride + i] (device, int32) names the page holding places [i, i + 1) * page_size of
  * sequence b; kv_lens[b] (device, int32) is its length in places INCLUDING this step's new tokens.  An id outside
- * [0, num_pages) holds no places: they are seen by nobody and nothing is written there.  Lengths are clamped to
- * [0, max_pages * page_size].
+ * [0, num_pages) holds no places: they are seen by nobody and nothing is written there, as are places >=
+ * max_pages * page_size of a longer sequence.
  * New tokens.  `tokens` rows are packed sequence after sequence: rows cu_seqlens[b] .. cu_seqlens[b + 1] (device, int32,
  * batch + 1 entries, ascending) belong to sequence b; with cu_seqlens == NULL every sequence brings tokens / batch of them.
  * Token i of the n_b of sequence b has place kv_lens[b] - n_b + i.  Rows outside every sequence are neither read nor written.

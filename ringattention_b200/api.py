@@ -421,6 +421,7 @@ def _workspace(p, size, workspace, device, where: str):
             workspace = torch.empty(int(n), dtype=torch.uint8, device=device)
     p.workspace, _ = _strided(workspace, "workspace", 1, (torch.uint8,), device)
     p.workspace_bytes = workspace.numel()
+    return workspace
 
 
 def paged_append(k, v, k_cache, v_cache, page_table, kv_lens, *, cu_seqlens=None, weights=None, stream=None) -> None:
@@ -495,8 +496,9 @@ def paged_attention_fwd(q, k_cache, v_cache, page_table, kv_lens, out, lse, *, c
     ctx, p.stream = _on(dev, stream)
     with ctx:
         lib = _lib.load()
-        _workspace(p, lib.ring_paged_attention_workspace, workspace, dev, "ring_paged_attention_fwd")
+        keep = _workspace(p, lib.ring_paged_attention_workspace, workspace, dev, "ring_paged_attention_fwd")
         check(lib.ring_paged_attention_fwd(ctypes.byref(p)), "ring_paged_attention_fwd")
+        del keep  # until here
 
 
 def paged_weights(weights, q, k_cache, lse, page_table, kv_lens, *, cu_seqlens=None, max_new: int = 0,
@@ -513,8 +515,9 @@ def paged_weights(weights, q, k_cache, lse, page_table, kv_lens, *, cu_seqlens=N
     ctx, p.stream = _on(k_cache.device, stream)
     with ctx:
         lib = _lib.load()
-        _workspace(p, lib.ring_paged_weights_workspace, workspace, k_cache.device, "ring_paged_weights")
+        keep = _workspace(p, lib.ring_paged_weights_workspace, workspace, k_cache.device, "ring_paged_weights")
         check(lib.ring_paged_weights(ctypes.byref(p)), "ring_paged_weights")
+        del keep  # until here
 
 
 def paged_evict(k_cache, v_cache, weights, page_table, kv_lens, dst_table, budget: int, new_lens, new_weights, kept, *,

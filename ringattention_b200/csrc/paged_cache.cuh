@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(256) ring_paged_append_kernel(const PagedAppen
             b = seq_of_token(a, t);
             if (b >= 0 && b < a.batch) {
                 const SeqView s = seq_view(a, b);
-                place = s.len - s.n + (t - s.q0);
+                place = s.pos + (t - s.q0);
                 if (t >= s.q0 && t < s.q0 + s.n && place >= 0) page = page_of(a, b, place >> a.page_shift);
             }
             slot = place & ((1 << a.page_shift) - 1);

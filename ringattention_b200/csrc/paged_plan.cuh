@@ -64,7 +64,8 @@ __device__ __forceinline__ int div_tokens(const PagedArgs& a, int x) {
 struct SeqView {
     int q0;   // first packed row
     int n;    // new tokens
-    int len;  // places, the new ones included
+    int len;  // places that exist: at most what the table's pages hold
+    int pos;  // place of the first new token, by the length as given (a place behind the table's pages does not exist)
 };
 
 __device__ __forceinline__ SeqView seq_view(const PagedArgs& a, int b) {
@@ -76,7 +77,9 @@ __device__ __forceinline__ SeqView seq_view(const PagedArgs& a, int b) {
         s.q0 = b * a.uniform_new;
         s.n = a.uniform_new;
     }
-    s.len = min(max(a.lens[b], 0), a.capacity);
+    const int given = max(a.lens[b], 0);
+    s.len = min(given, a.capacity);
+    s.pos = given - s.n;
     return s;
 }
 
@@ -89,10 +92,10 @@ __device__ __forceinline__ int page_of(const PagedArgs& a, int b, int i) {
 
 // Places a token of the sequence sees: [0, hi) without [sinks, lo).
 __device__ __forceinline__ int token_hi(const PagedArgs& a, const SeqView& s, int token) {
-    return a.causal ? min(max(s.len - s.n + token + 1, 0), s.len) : s.len;
+    return a.causal ? min(max(s.pos + token + 1, 0), s.len) : s.len;
 }
 __device__ __forceinline__ int token_lo(const PagedArgs& a, const SeqView& s, int token) {
-    return a.window > 0 ? max(s.len - s.n + token - a.window + 1, 0) : 0;
+    return a.window > 0 ? max(s.pos + token - a.window + 1, 0) : 0;
 }
 
 // The key blocks of BN places a tile of query rows has to visit: blocks [0, sink) and then [first, ...), count in all.

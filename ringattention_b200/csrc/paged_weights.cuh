@@ -268,9 +268,9 @@ struct WeightsChunkUnits {
     static __device__ __forceinline__ void range(const PagedArgs& a, const SeqView& s, int tile, int* j0, int* first, int* count) {
         *j0 = seen_tiles<256>(a, s).block(tile) * 256;
         int t0 = 0, t1 = s.n;
-        if (a.causal) t0 = max(0, *j0 - (s.len - s.n));
+        if (a.causal) t0 = max(0, *j0 - s.pos);
         if (a.window > 0 && *j0 >= a.sinks)
-            t1 = static_cast<int>(min(static_cast<int64_t>(s.n), static_cast<int64_t>(*j0) + 255 + a.window - (s.len - s.n)));
+            t1 = static_cast<int>(min(static_cast<int64_t>(s.n), static_cast<int64_t>(*j0) + 255 + a.window - s.pos));
         *first = div_tokens(a, min(t0, s.n - 1));
         *count = max(div_tokens(a, max(t1, 0) + a.row_tokens - 1) - *first, 1);
     }
@@ -513,7 +513,7 @@ ring_paged_weights_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const 
                 // before the first whose window has left it.
                 int c0 = 0, c1 = 0;
                 if (edge) {
-                    const int back = j - (s.len - s.n) - t0;  // the place as an index into the tile's tokens
+                    const int back = j - s.pos - t0;  // the place as an index into the tile's tokens
                     c1 = min(t1 - t0, a.row_tokens);
                     if (a.causal) c0 = min(max(back, 0), a.row_tokens) * a.group;
                     if (a.window > 0 && j >= a.sinks)

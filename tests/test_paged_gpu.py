@@ -122,13 +122,55 @@ def test_pages_that_do_not_exist_hold_no_places(ops, name, wrong):
     assert bool(((s.weights.cpu().double() - w).abs() <= tol).all())
 
 
-def test_lengths_beyond_the_table_are_clamped(ops):
-    s = Setup([40, 30], [1, 1], extra_cols=0, ragged=False, page=8)
-    s.kv_lens[0] = 1_000_000
+@pytest.mark.parametrize("new", [1, 40])
+def test_places_behind_the_table_do_not_exist(ops, new):
+    s = Setup([40, 40], [new, new], extra_cols=0, ragged=False, page=8)
+    s.kv_lens[0] = (1 << 31) - 1
     s.kv_lens[1] = -5
     got = attend(ops, s)
     s.lens = [s.table.shape[1] * s.page, 0]
-    check_attention(s, got, attention_ref(s))
+    check_attention(s, got, attention_ref(s, causal=False) if new > 1 else attention_ref(s))
+    # new tokens whose places do not exist go nowhere, those in front of them to their own
+    s.kv_lens[0] = 45
+    k, v, w = s.k_cache.clone(), s.v_cache.clone(), s.weights.clone()
+    for i in range(new):
+        j = 45 - new + i
+        if j < 40:
+            pg = int(s.table[0, j // 8])
+            k[pg, :, j % 8], v[pg, :, j % 8], w[0, :, j] = s.k_new[i], s.v_new[i], 0.0
+    ops.paged_append(s.k_new, s.v_new, s.k_cache, s.v_cache, s.table, s.kv_lens, weights=s.weights)
+    assert torch.equal(k, s.k_cache) and torch.equal(v, s.v_cache) and torch.equal(w, s.weights)
+    got = attend(ops, s, window=30, sinks=2)
+    p = torch.arange(new)[:, None] + 45 - new
+    j = torch.arange(40)[None]
+    see = (j <= p) & ((j > p - 30) | (j < 2))
+    for h in range(4):
+        x = s.q[:new, h].cpu().double() @ s.rows(s.k_cache, 0, h // 2)[0].T / 8.0
+        want = torch.softmax(x.masked_fill(~see, -math.inf), dim=1) @ s.rows(s.v_cache, 0, h // 2)[0]
+        # fp16: P and out by half a step each, scores as in check_attention, all below 2^-9 of the largest |v|
+        assert float((got[0][:new, h].cpu().double() - want).abs().max()) <= 2.0 ** -9 * float(s.v_cache.abs().max())
+
+
+def test_two_threads_share_a_stream(ops):
+    """Calls from two host threads on one stream: every call has scratch of its own."""
+    import threading
+    s, t = Setup([700], [1], dim=128, group=4, ragged=False), Setup([900, 300], [200, 90], dim=128, group=4, seed=2)
+    want = [attend(ops, s), attend(ops, t)]
+    stream, bad = torch.cuda.current_stream(), []
+
+    def work(x, w):
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got = attend(ops, x)
+                if not (torch.equal(got[0], w[0]) and torch.equal(got[1], w[1])):
+                    bad.append(1)
+
+    threads = [threading.Thread(target=work, args=a) for a in ((s, want[0]), (t, want[1]))]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not bad
 
 
 def test_strided_operands(ops):
