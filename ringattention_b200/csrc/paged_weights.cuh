@@ -9,9 +9,10 @@
 // MUFU does 16 exponentials a clock: 2048 clocks against 1024 of tensor time at D = 128, so the exponentials bound it.  S^T = K Q^T
 // with the places as TMEM lanes: a thread owns one place, its sum over the columns stays in a register, nothing crosses threads.
 //
-// Measured: rows form, 16 sequences of 500 to 8192 places, 8 K/V heads, group 4, D = 128, one token: 37 us, 4.1 TB/s (launch, plan and the
-// last steps are a third of it).  Chunk form, 1024 tokens over 8192 places, 32 / 8 heads, D = 128: 102 us, about 2500 clocks a block
-// against the 2048 of the exponentials; moving a quarter of them to the FMA pipe: 105 -> 102 us, half: 107.
+// Measured: rows form, 16 sequences of 500 to 8192 places, 8 K/V heads, group 4, D = 128, one token: 36 us, 4.1 TB/s (launch, plan and the
+// last steps are a third of it).  Chunk form, 1024 tokens over 8192 places, 32 / 8 heads, D = 128: 99 us, about 2500 clocks a block
+// against the 2048 of the exponentials; moving a quarter of them to the FMA pipe took
+// 105 us to 102, half to 107.
 #pragma once
 
 #include <cstdint>
@@ -127,6 +128,8 @@ __global__ void __launch_bounds__(T::kThreads) ring_paged_weights_rows_kernel(co
         float* wrow = a.weights + static_cast<int64_t>(g.b) * a.w_batch + static_cast<int64_t>(g.h) * a.w_head;
         int ids_next = -1;
         uint32_t have = 0, seen = 0;
+        float old_next[KT / 32] = {};
+        bool put_next[KT / 32] = {};
 #pragma unroll 1
         for (int i = -kAhead; i < g.count; ++i) {
             const int n = i + kAhead;
@@ -157,20 +160,25 @@ __global__ void __launch_bounds__(T::kThreads) ring_paged_weights_rows_kernel(co
                 }
             }
             cp_async_commit();
+            // a lane's places of a step's result are 32 u + lane of it; their old weights are fetched a step ahead
+            float old[KT / 32];
+            bool put[KT / 32];
+#pragma unroll
+            for (int u = 0; u < KT / 32; ++u) {
+                old[u] = old_next[u];
+                put[u] = put_next[u];
+                put_next[u] = false;
+                if (i + 1 >= 0 && i + 1 < g.count) {
+                    const int j = place_of(i + 1) + 32 * u + lane;
+                    put_next[u] = j < hi_max && (j >= lo_min || j < a.sinks) && ((seen >> (NG + 4 * u + (lane >> 3))) & 1u);
+                    if (put_next[u]) old_next[u] = wrow[j];
+                }
+            }
             if (i < 0) {
                 seen >>= NG;
                 continue;
             }
             const int j0 = place_of(i);
-            // a lane's places of the result are j0 + 32 u + lane; their old weights travel while the step is computed
-            float old[KT / 32];
-            bool put[KT / 32];
-#pragma unroll
-            for (int u = 0; u < KT / 32; ++u) {
-                const int j = j0 + 32 * u + lane;
-                put[u] = j < hi_max && (j >= lo_min || j < a.sinks) && ((seen >> (4 * u + (lane >> 3))) & 1u);
-                old[u] = put[u] ? wrow[j] : 0.f;
-            }
             cp_async_wait<kAhead>();
             __syncwarp();
             const uint32_t kst = ring + (i % T::kStages) * T::kStageBytes;
