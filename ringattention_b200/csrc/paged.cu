@@ -135,7 +135,7 @@ void query_args(const Ring_paged_params& p, ring::PagedArgs* a) {
     a->scale_log2 = p.softmax_scale * 1.4426950408889634f;
     a->causal = p.causal ? 1 : 0;
     a->window = p.window < (1 << 30) ? p.window : 1 << 30;  // no sequence is longer: the same mask, and no sum overflows
-    a->sinks = p.sinks;
+    a->sinks = p.sinks < (1 << 30) ? p.sinks : 1 << 30;
     a->weights = p.weights;
     a->w_batch = p.weights_batch_stride;
     a->w_head = p.weights_head_stride;

@@ -334,8 +334,8 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                                 for (int bx = 0; bx < kBoxes; ++bx) st_shared_v4(to + bx * kBoxBytes + r * 128, 0u, 0u, 0u, 0u);
                             }
                         };
-                        clear(max(hi_max - j0, 0), BN);
-                        clear(max(a.sinks - j0, 0), min(lo_min - j0, BN));
+                        clear(min(max(hi_max - j0, 0), BN), BN);
+                        clear(min(max(a.sinks - j0, 0), BN), min(lo_min - j0, BN));
                         fence_proxy_async_cta();
                         __syncwarp();
                     }

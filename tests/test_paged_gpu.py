@@ -46,6 +46,9 @@ CASES = {
     "chunk_g40": ([300, 90], [30, 11], dict(kv_heads=1, group=40, dtype="bf16")),
     "chunk_g130": ([200], [3], dict(kv_heads=1, group=130, page=32)),
     "long_chunk": ([5000, 1300], [700, 33], dict(kv_heads=1, group=2, page=64, dtype="bf16")),
+    "one_head_one_page": ([300], [100], dict(kv_heads=1, group=1, page=512, spare_pages=0, extra_cols=0, dtype="bf16")),
+    "many_sequences_one_long": ([740] + [(13 * i) % 60 for i in range(44)], [700] + [(13 * i) % 60 % 7 for i in range(44)],
+                                dict(kv_heads=1, group=2, page=16)),
     "page_above_tile": ([900, 513], [70, 200], dict(group=2, page=512, dim=128)),
 }
 
@@ -70,6 +73,32 @@ def test_attention_fp32_out_scale_and_hint(ops, name):
     check_attention(s, got, want, out_type=torch.float32, what=name)
     for hint in (1, 0, 10_000):  # a wrong hint chooses another kernel, not another result
         check_attention(s, attend(ops, s, fp32_out=True, softmax_scale=0.2, max_new=hint), want, out_type=torch.float32, what=f"{name} {hint}")
+
+
+@pytest.mark.parametrize("name", ["decode_d128_g4", "few_tokens_g5", "chunk_g7"])
+def test_attention_extreme_masks(ops, name):
+    """Windows and first tokens beyond any sequence are no mask; a window of one place and no first tokens is the token itself."""
+    lens, news, kw = CASES[name]
+    s = Setup(lens, news, seed=13, **kw)
+    want = attention_ref(s)
+    for m in (dict(window=(1 << 31) - 1), dict(window=1, sinks=(1 << 31) - 1), dict(window=1 << 30, sinks=7)):
+        check_attention(s, attend(ops, s, **m), want, what=str(m))
+        lse = want[1].float().cuda()
+        w, tol = weights_ref(s, lse)
+        got = s.weights.clone()
+        ops.paged_weights_(got, s.q, s.k_cache, lse, s.table, s.kv_lens, cu_seqlens=s.cu, max_new=s.max_new, **m)
+        assert bool(((got.cpu().double() - w).abs() <= tol).all())
+    check_attention(s, attend(ops, s, window=1), attention_ref(s, window=1))
+
+
+@pytest.mark.parametrize("name", ["decode_d128_g4", "chunk_g4_d128"])
+def test_keys_and_values_laid_out_differently(ops, name):
+    lens, news, kw = CASES[name]
+    s = Setup(lens, news, seed=14, **kw)
+    v = torch.empty((s.pages, s.page, s.kv_heads, s.dim), dtype=s.dtype, device="cuda").transpose(1, 2)
+    v.copy_(s.v_cache)
+    got = ops.paged_attention(s.q, s.k_cache, v, s.table, s.kv_lens, cu_seqlens=s.cu, max_new=s.max_new)
+    check_attention(s, got, attention_ref(s))
 
 
 @pytest.mark.parametrize("name", ["decode_d128_g4", "chunk_g4_d128"])
