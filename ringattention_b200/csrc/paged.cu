@@ -479,6 +479,8 @@ int ring_paged_evict(const Ring_evict_params* params) {
     PAGED_REQUIRE(p.new_lens != p.kv_lens, "new_lens must not be kv_lens");
     PAGED_REQUIRE(p.weights_len >= static_cast<int64_t>(p.max_pages) * p.page_size, "weights_len must be at least max_pages * page_size");
     PAGED_REQUIRE(p.new_weights_len >= p.budget, "new_weights_len must be at least budget");
+    // loops over these step past their end by up to a block: far from where 32 bits turn over
+    PAGED_REQUIRE(p.new_weights_len <= (1 << 30) && p.budget <= (1 << 30), "budget and new_weights_len must not exceed 2^30");
     PAGED_REQUIRE(p.weights_batch_stride >= 0 && p.weights_head_stride >= 0 && p.new_weights_batch_stride >= 0 &&
                       p.new_weights_head_stride >= 0, "weights strides must not be negative");
     ring::PagedEvictArgs e;

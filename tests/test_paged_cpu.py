@@ -97,6 +97,8 @@ def test_paged_calls_refuse(lib, fn, kw, needle):
     (dict(new_weights=0xa000), "must not be weights"), (dict(kept=None), "kept"), (dict(new_lens=0x4000), "kv_lens"),
     (dict(weights_len=63), "weights_len"), (dict(new_weights_len=31), "new_weights_len"), (dict(v_place_stride=0), "strides of 0"),
     (dict(v_cache=None), "v_cache"), (dict(recent=(1 << 31) - 1, first=2), "at most budget"),
+    (dict(budget=(1 << 30) + 1, dst_pages=1 << 27, dst_stride=1 << 27, new_weights_len=(1 << 31) - 1), "2^30"),
+    (dict(new_weights_len=(1 << 31) - 1), "2^30"),
 ])
 def test_evict_refuses(lib, kw, needle):
     p = evict(**kw)
