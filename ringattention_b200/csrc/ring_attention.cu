@@ -150,6 +150,15 @@ int device_state(DeviceState** out) {
 
 // ------------------------------------------------------------------------------------------ tensor maps
 int encode_fn(EncodeTiledFn* out) {
+    // The encoder is a driver call and needs a context that is current: a host thread that has made no runtime call of the
+    // binding kind yet (its memory may all have come from a caching allocator) has none, and cudaSetDevice binds one.
+    static thread_local bool bound = false;
+    if (!bound) {
+        int dev = 0;
+        RING_CUDA(cudaGetDevice(&dev));
+        RING_CUDA(cudaSetDevice(dev));
+        bound = true;
+    }
     static EncodeTiledFn fn = nullptr;
     static std::mutex m;
     std::lock_guard<std::mutex> lock(m);

@@ -188,11 +188,14 @@ def test_two_threads_share_a_stream(ops):
     stream, bad = torch.cuda.current_stream(), []
 
     def work(x, w):
-        with torch.cuda.stream(stream):
-            for _ in range(20):
-                got = attend(ops, x)
-                if not (torch.equal(got[0], w[0]) and torch.equal(got[1], w[1])):
-                    bad.append(1)
+        try:
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    got = attend(ops, x)
+                    if not (torch.equal(got[0], w[0]) and torch.equal(got[1], w[1])):
+                        bad.append("differs")
+        except Exception as e:  # an exception ends the thread, not the test
+            bad.append(repr(e))
 
     threads = [threading.Thread(target=work, args=a) for a in ((s, want[0]), (t, want[1]))]
     for th in threads:
@@ -200,6 +203,36 @@ def test_two_threads_share_a_stream(ops):
     for th in threads:
         th.join()
     assert not bad
+
+
+def test_first_call_of_a_host_thread(ops):
+    """A new thread's first CUDA call of any kind is one of these (no context is current in it yet)."""
+    import threading
+    from ringattention_b200 import torch_ops
+    s = Setup([900, 300], [200, 90], dim=128, group=4, seed=2)
+    out, lse = attend(ops, s)
+    w = s.weights.clone()
+    ops.paged_weights_(w, s.q, s.k_cache, lse, s.table, s.kv_lens, cu_seqlens=s.cu, max_new=s.max_new)
+    q = torch.randn((1, 2, 256, 128), device="cuda").half()
+    whole = torch_ops.block_forward(q, q, q)
+    torch.cuda.synchronize()
+    got = {}
+
+    def run(name, f):
+        try:
+            got[name] = f()
+        except Exception as e:
+            got[name] = e
+
+    calls = {"attention": lambda: attend(ops, s), "block": lambda: torch_ops.block_forward(q, q, q),
+             "weights": lambda: ops.paged_weights_(s.weights, s.q, s.k_cache, lse, s.table, s.kv_lens, cu_seqlens=s.cu, max_new=s.max_new)}
+    for name, f in calls.items():
+        th = threading.Thread(target=run, args=(name, f))
+        th.start()
+        th.join()
+    torch.cuda.synchronize()
+    assert not [v for v in got.values() if isinstance(v, Exception)], got
+    assert torch.equal(got["attention"][0], out) and torch.equal(got["block"][0], whole[0]) and torch.equal(s.weights, w)
 
 
 def test_strided_operands(ops):
