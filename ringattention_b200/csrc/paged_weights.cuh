@@ -555,7 +555,7 @@ ring_paged_weights_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const 
                         ffma2(x0, x1, sc[v], sc[v + 1], c, c, nl.x, nl.y);
                         ffma2(x2, x3, sc[v + 2], sc[v + 3], c, c, nl.z, nl.w);
                         if (v % T::kPolyEvery == 0)
-                            ex2_poly2(x0, x1, x0, x1);
+                            ex2_poly2<true>(x0, x1, x0, x1);
                         else
                             x0 = ex2_approx(x0), x1 = ex2_approx(x1);
                         fadd2(a0, a1, a0, a1, x0, x1);
