@@ -262,7 +262,7 @@ struct PagedWeightsTraits : public Ring_kernel_traits<kHeadDim_, 256, 128, 12, e
     static constexpr int kKSlots = 2;                         // the next unit's places load while this one's are used
     static constexpr int kQSlots = kHeadDim == 128 ? 2 : 4;
     static constexpr int kSmemTiles = (2 * kKSlots + kQSlots) * kTileBytes;
-    static constexpr int kRowInfo = kQRows * 4;               // negated lse (base 2) of each row
+    static constexpr int kRowInfo = 2 * kQRows * 4 + 16;      // negated lse (base 2) of each row, the same with 0 for NaN, a bit per NaN
     static constexpr int kPolyEvery = 8;                      // of 8 columns 2 are evaluated on the FMA pipe
     static constexpr int kInfoSlots = 4;                      // a ring of its own: read until a block's sums are done, long after its tile
     static constexpr int kNumBarriers = 2 * kKSlots + 2 * kQSlots + 4 /*s_full*/ + 4 /*s_free*/ + 2 * kInfoSlots;
@@ -288,6 +288,24 @@ struct WeightsChunkUnits {
         return count;
     }
 };
+
+// Makes the scores of the rows (columns of S^T) whose bit is set NaN where they are, in TMEM.  By a warp, for its lanes; a call, so that
+// the summing loop does not carry it (as a part of that loop it cost 7 us of 99).
+__device__ __noinline__ void nan_scores(uint32_t t_s, float4 rows) {
+    using namespace ptx;
+#pragma unroll 1
+    for (int w = 0; w < 4; ++w) {
+        const uint32_t bits = __float_as_uint(w == 0 ? rows.x : (w == 1 ? rows.y : (w == 2 ? rows.z : rows.w)));
+        uint32_t x[32];
+        tmem_ld_x32(t_s + 32 * w, x);
+        tmem_wait_ld();
+#pragma unroll
+        for (int v = 0; v < 32; ++v)
+            if ((bits >> v) & 1u) x[v] = 0x7fffffffu;
+        tmem_st_x32(t_s + 32 * w, x);
+    }
+    tmem_wait_st();
+}
 
 template <class T>
 __global__ void __launch_bounds__(T::kNThreads, 1)
@@ -434,6 +452,7 @@ ring_paged_weights_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const 
                     const int q = blocks % T::kInfoSlots;
                     const int t0 = (q_first + g.first + i) * a.row_tokens;
                     float nl[4];
+                    uint32_t nan[4];
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {  // the loads do not wait for the slot
                         const int r = lane + 32 * u, dt = div_group(a, r);
@@ -442,6 +461,7 @@ ring_paged_weights_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const 
                             const float l = a.lse[static_cast<int64_t>(s.q0 + t0 + dt) * a.heads + g.h * a.group + (r - dt * a.group)];
                             if (l != -INFINITY) nl[u] = -l * 1.4426950408889634f;
                         }
+                        nan[u] = __ballot_sync(0xffffffffu, nl[u] != nl[u]);
                     }
                     if (blocks >= T::kInfoSlots) {
                         ok = mbar_wait(bar_i_empty(q), (blocks / T::kInfoSlots - 1) & 1, abort_flag, a.status, kDevPagedLoad);
@@ -450,7 +470,11 @@ ring_paged_weights_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const 
                     }
                     float* info = row_info(q);
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) info[lane + 32 * u] = nl[u];
+                    for (int u = 0; u < 4; ++u) {
+                        info[lane + 32 * u] = nl[u];
+                        info[T::kQRows + lane + 32 * u] = nl[u] != nl[u] ? 0.f : nl[u];
+                        if (lane == 0) reinterpret_cast<uint32_t*>(info + 2 * T::kQRows)[u] = nan[u];
+                    }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar_i_full(q));
                 }
@@ -514,9 +538,18 @@ ring_paged_weights_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const 
                 const int q = blocks % T::kInfoSlots, buf = blocks & 1;
                 if (i == 0 && !(ok = acquire())) break;
                 const int t0 = (q_first + g.first + i) * a.row_tokens, t1 = min(t0 + a.row_tokens, s.n);
-                const uint32_t info = smem_u32(row_info(q));
                 const bool edge = t0 + a.row_tokens > s.n || jt + 128 > token_hi(a, s, t0) ||
                                   (token_lo(a, s, t1 - 1) > jt && jt + 128 > a.sinks);
+                uint32_t info = smem_u32(row_info(q));
+                if (edge) {
+                    const float4 nan = ld_shared_v4(info + 2 * T::kQRows * 4);
+                    if ((__float_as_uint(nan.x) | __float_as_uint(nan.y) | __float_as_uint(nan.z) | __float_as_uint(nan.w)) != 0) {
+                        tmem_wait_ld();
+                        nan_scores(t_s + buf * 128, nan);
+                        tmem_ld_x32(t_s + buf * 128, sr[0]);
+                        info += T::kQRows * 4;
+                    }
+                }
                 // The columns whose token sees this place are one interval: behind the first token at or after the place (causal),
                 // before the first whose window has left it.
                 int c0 = 0, c1 = 0;

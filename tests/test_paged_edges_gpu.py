@@ -85,9 +85,9 @@ def test_rows_without_lse_add_nothing(ops, name):
 
 
 @pytest.mark.parametrize("name", ["rows_g1_d64", "chunk_g1_d64", "chunk_g4_d128", "chunk_g7_d128"])
-@pytest.mark.parametrize("where", ["q"])
+@pytest.mark.parametrize("where", ["q", "lse", "q and lse"])
 def test_weights_keep_a_nan_row_visible(ops, name, where):
-    """A NaN query row makes every place that its token sees NaN, and no other, whichever column of a tile it is."""
+    """A NaN query row, or a NaN lse, makes every place that its token sees NaN, and no other, whichever column of a tile it is."""
     lens, news, kw = TRACKED[name]
     s = Setup(lens, news, seed=44, **kw)
     lse = attention_ref(s)[1].float().cuda()
@@ -95,9 +95,9 @@ def test_weights_keep_a_nan_row_visible(ops, name, where):
     for i in range(8):
         tok, head = min(9 + i, news[0] - 1), (3 * i) % heads
         q, l = s.q.clone(), lse.clone()
-        if where == "q":
+        if "q" in where:
             q[tok, head, i] = math.nan
-        else:
+        if "lse" in where:
             l[tok, head] = math.nan
         got = weigh(ops, s, s.weights.clone(), l, q=q).cpu()
         want = torch.zeros(got.shape, dtype=torch.bool)
