@@ -95,7 +95,8 @@ __device__ __forceinline__ int token_hi(const PagedArgs& a, const SeqView& s, in
     return a.causal ? min(max(s.pos + token + 1, 0), s.len) : s.len;
 }
 __device__ __forceinline__ int token_lo(const PagedArgs& a, const SeqView& s, int token) {
-    return a.window > 0 ? max(s.pos + token - a.window + 1, 0) : 0;
+    // at most len, or the blocks of a window far behind the table's pages would lie where 32 bits turn over
+    return a.window > 0 ? min(max(s.pos + token - a.window + 1, 0), s.len) : 0;
 }
 
 // The key blocks of BN places a tile of query rows has to visit: blocks [0, sink) and then [first, ...), count in all.

@@ -103,3 +103,28 @@ def test_weights_keep_a_nan_row_visible(ops, name, where):
         want = torch.zeros(got.shape, dtype=torch.bool)
         want[0, head // s.group, :lens[0] - news[0] + tok + 1] = True
         assert torch.equal(torch.isnan(got), want), (tok, head)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("back", [1, 5, 127, 128, 129, 300])
+def test_windows_of_lengths_near_the_end_of_32_bits(ops, new, dim, back):
+    """A length far behind what the table's pages hold: the window lies where no places are, and only the first tokens are seen."""
+    s = Setup([40, 40], [new, new], dim=dim, extra_cols=0, ragged=False, page=8, seed=back)
+    s.kv_lens[0] = (1 << 31) - back
+    for sinks in (0, 2):
+        m = dict(window=30, sinks=sinks)
+        out, lse = (x.cpu() for x in attend(ops, s, **m))
+        got = weigh(ops, s, s.weights.clone(), lse.cuda(), **m).cpu()
+        t = Setup([sinks, 40], [new, new], dim=dim, ragged=False, page=8)
+        t.q, t.k_cache, t.v_cache, t.table, t.weights, t.pages = s.q, s.k_cache, s.v_cache, s.table, s.weights, s.pages
+        # sequence 0 as one of `sinks` places that all its tokens see, sequence 1 with its own mask
+        far, near = attention_ref(t, causal=False), attention_ref(t, **m)
+        want = [torch.cat([f[:new], n[new:]]) for f, n in zip(far, near)]
+        check_attention(t, (out, lse), want, what=f"{sinks}")
+        wf, tf = weights_ref(t, lse, causal=False)
+        wn, tn = weights_ref(t, lse, **m)
+        err = torch.cat([(got.double() - wf).abs()[:1] / tf[:1], (got.double() - wn).abs()[1:] / tn[1:]])
+        assert bool((err <= 1).all()), f"{sinks}: {err.max():.2f} times the bound"
+        if sinks == 0:
+            assert torch.equal(got[0], s.weights[0].cpu())
