@@ -128,3 +128,153 @@ def test_windows_of_lengths_near_the_end_of_32_bits(ops, new, dim, back):
         assert bool((err <= 1).all()), f"{sinks}: {err.max():.2f} times the bound"
         if sinks == 0:
             assert torch.equal(got[0], s.weights[0].cpu())
+
+
+# The forms change at 9, 17 and 33 query rows a K/V head: (group, new tokens of the longest) on both sides of each, and between
+FORM_ROWS = {8: (8, 1), 9: (3, 3), 16: (4, 4), 17: (1, 17), 24: (8, 3), 31: (1, 31), 32: (4, 8), 33: (3, 11)}
+
+
+@pytest.mark.parametrize("rows", FORM_ROWS)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_both_sides_of_every_choice_of_form(ops, rows, dim, dtype):
+    """Units cut into few and into many partials, units of fewer rows, pages that do not exist, windows; attention and weights."""
+    group, new = FORM_ROWS[rows]
+    s = Setup([2900, 500, 64, 0], [new, max(new - 1, 1), 1, 0], dim=dim, dtype=dtype, group=group, page=16, seed=rows)
+    s.table[0, 3], s.table[1, 30] = -1, s.pages
+    for m in (dict(), dict(causal=False), dict(window=1200, sinks=40)):
+        want = attention_ref(s, **m)
+        got = attend(ops, s, **m)
+        check_attention(s, got, want, what=str(m))
+        lse = want[1].float().cuda()
+        w, tol = weights_ref(s, lse, **m)
+        once, again = weigh(ops, s, s.weights.clone(), lse, **m), weigh(ops, s, s.weights.clone(), lse, **m)
+        assert bool(((once.cpu().double() - w).abs() <= tol).all()), str(m)
+        repeat = attend(ops, s, **m)
+        assert torch.equal(once, again) and torch.equal(got[0], repeat[0]) and torch.equal(got[1], repeat[1])
+
+
+@pytest.mark.parametrize("rows", [16, 24, 32])
+@pytest.mark.parametrize("dim,dtype", [(64, "fp16"), (64, "bf16"), (128, "bf16")])
+def test_one_long_sequence_in_every_share(ops, rows, dim, dtype):
+    group, new = FORM_ROWS[rows]
+    s = Setup([40000], [new], dim=dim, dtype=dtype, group=group, kv_heads=1, page=64, layout="NHD", seed=rows)
+    want = attention_ref(s)
+    got = attend(ops, s)
+    check_attention(s, got, want)
+    w, tol = weights_ref(s, got[1])
+    assert bool(((weigh(ops, s, s.weights.clone(), got[1]).cpu().double() - w).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("name", TRACKED)
+def test_weights_with_a_window_and_no_first_tokens(ops, name):
+    lens, news, kw = TRACKED[name]
+    s = Setup(lens, news, seed=47, **kw)
+    for window in (1, 64, 300):
+        lse = attention_ref(s, window=window)[1].float().cuda()
+        want, tol = weights_ref(s, lse, window=window)
+        got = weigh(ops, s, s.weights.clone(), lse, window=window)
+        assert bool(((got.cpu().double() - want).abs() <= tol).all()), window
+
+
+@pytest.mark.parametrize("group,dim", [(4, 128), (1, 64), (7, 128)])
+def test_query_strides_on_the_tensor_map_forms(ops, group, dim):
+    """q as a slice of a wider projection, of a transposed one, and the head dimension padded: the same bits as contiguous rows."""
+    s = Setup([700, 300], [150, 64], group=group, dim=dim, dtype="bf16", page=64, seed=48)
+    heads = s.kv_heads * group
+    want = attend(ops, s)
+    w = weigh(ops, s, s.weights.clone(), want[1])
+    wide = torch.full((s.tokens, heads + 5, dim), math.nan, dtype=s.dtype, device="cuda")
+    turned = torch.full((heads, s.tokens + 3, dim), math.nan, dtype=s.dtype, device="cuda")
+    padded = torch.full((s.tokens, heads, dim + 8), math.nan, dtype=s.dtype, device="cuda")
+    for q in (wide[:, 2:2 + heads], turned[:, 1:1 + s.tokens].transpose(0, 1), padded[:, :, :dim]):
+        q.copy_(s.q)
+        got = ops.paged_attention(q, s.k_cache, s.v_cache, s.table, s.kv_lens, cu_seqlens=s.cu, max_new=s.max_new)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        assert torch.equal(weigh(ops, s, s.weights.clone(), want[1], q=q), w)
+
+
+def test_overlapping_graphs_leave_what_eager_calls_leave(ops):
+    """Append, attention and weights captured, replayed on two streams at once: cache, weights, out and lse are those of eager calls."""
+    sets = [Setup([100, 257], [1, 1], dim=128, group=4, dtype="bf16", ragged=False), Setup([400, 300], [90, 120], dim=128, group=4, dtype="bf16", seed=2),
+            Setup([600], [40], group=1, seed=3)]
+
+    def step(x):
+        ops.paged_append(x.k_new, x.v_new, x.k_cache, x.v_cache, x.table, x.kv_lens, cu_seqlens=x.cu, weights=x.weights)
+        got = attend(ops, x)
+        weigh(ops, x, x.weights, got[1])
+        return got
+
+    def contents(x):
+        return [x.k_cache, x.v_cache, x.weights]
+
+    first = [[c.clone() for c in contents(x)] for x in sets]
+
+    def reset():
+        for x, f in zip(sets, first):
+            for c, old in zip(contents(x), f):
+                c.copy_(old)
+        torch.cuda.synchronize()
+
+    for x in sets:
+        step(x)
+    torch.cuda.synchronize()
+    graphs = []
+    for x in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step(x)
+        graphs.append((g, out))
+    streams = [torch.cuda.Stream() for _ in sets]
+    for lens in ([100, 257], [64, 130], [1, 2]):
+        sets[0].kv_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        reset()
+        want = []
+        for x in sets:
+            for _ in range(3):
+                got = step(x)
+            want.append([c.clone() for c in contents(x) + list(got)])
+        reset()
+        for _ in range(3):
+            for (g, _), st in zip(graphs, streams):
+                with torch.cuda.stream(st):
+                    g.replay()
+        torch.cuda.synchronize()
+        for x, (_, out), ref in zip(sets, graphs, want):
+            for c, r in zip(contents(x) + list(out), ref):
+                assert torch.equal(c, r), str(lens)
+
+
+@pytest.mark.parametrize("dtype,dim", [("fp16", 64), ("bf16", 128)])
+def test_rows_of_a_ring_forward_become_the_cache(ops, dtype, dim):
+    """A prompt goes through the ring on two virtual ranks, its K and V into pages; a chunk's attention gives the same rows, and a token
+    then answers over the cache."""
+    from ringattention_b200 import RingContext
+    s = Setup([512, 512], [512, 512], dim=dim, dtype=dtype, group=1, kv_heads=3, page=32, ragged=False, seed=49)
+    b, h, n = 2, 3, 512
+    q, k, v = (x.reshape(b, n, h, dim).transpose(1, 2).contiguous() for x in (s.q, s.k_new, s.v_new))
+    ctx = RingContext.create_local(2)
+    half = n // 2
+    shards = [[x[:, :, r * half:(r + 1) * half].contiguous() for r in range(2)] for x in (q, k, v)]
+    ctx.set_local_shards(shards[1], shards[2])
+    parts = [ops.ring_forward(ctx, shards[0][r], shards[1][r], shards[2][r], causal=True, mype=r) for r in range(2)]
+    ctx.synchronize()
+    torch.cuda.synchronize()
+    # the shards' rows go to the cache shard after shard, the lengths growing with them
+    for r in range(2):
+        lens = torch.full((2,), (r + 1) * half, dtype=torch.int32, device="cuda")
+        kr, vr = (torch.cat([x[i].transpose(0, 1) for i in range(b)]) for x in (shards[1][r], shards[2][r]))
+        ops.paged_append(kr, vr, s.k_cache, s.v_cache, s.table, lens)
+    want = attention_ref(s)
+    ring = [torch.cat([p[i] for p in parts], dim=2) for i in range(2)]
+    ring = ring[0].transpose(1, 2).reshape(b * n, h, dim), ring[1].transpose(1, 2).reshape(b * n, h)
+    check_attention(s, ring, want, out_type=torch.float32, what="ring")
+    check_attention(s, attend(ops, s), want, what="paged")
+    # one more token each, in a page of its own behind the prompt's
+    t = Setup([513, 513], [1, 1], dim=dim, dtype=dtype, group=1, kv_heads=3, page=32, ragged=False, seed=50, extra_cols=0, spare_pages=s.pages)
+    t.k_cache[:s.pages], t.v_cache[:s.pages] = s.k_cache, s.v_cache
+    t.table[:, :16] = s.table[:, :16]
+    t.table[:, 16] = torch.tensor([s.pages, s.pages + 1])
+    ops.paged_append(t.k_new, t.v_new, t.k_cache, t.v_cache, t.table, t.kv_lens)
+    check_attention(t, attend(ops, t), attention_ref(t), what="next token")
+    ctx.destroy()
