@@ -267,7 +267,7 @@ int ring_static_status(int* status_out, void* stream);
  * New tokens.  `tokens` rows are packed sequence after sequence: rows cu_seqlens[b] .. cu_seqlens[b + 1] (device, int32,
  * batch + 1 entries, ascending) belong to sequence b; with cu_seqlens == NULL every sequence brings tokens / batch of them.
  * Token i of the n_b of sequence b has place kv_lens[b] - n_b + i.  Rows outside every sequence are neither read nor written.
- * max_new is an upper bound on n_b, used to choose a kernel (0: tokens); results stay right if it is too small.
+ * max_new is an upper bound on n_b, used to choose ONE kernel for the whole call (0: tokens); results stay right if it is too small.
  * The lengths stay on the device: no call waits for the GPU, allocates or keeps anything between calls, so calls may be captured
  * into graphs and overlap (each with a workspace of its own).  As everywhere in this library, the first call on a
  * device does its one-time set-up; make it before any stream capture.  All of it runs on the current device.
@@ -335,7 +335,9 @@ int64_t ring_paged_attention_workspace(const Ring_paged_params* params);
 /*
  * Adds to the weight of every place what the new tokens' attention gave it:
  *   weights[b, h, j] += sum_i sum_g exp(s_ig,j - lse_ig)     i: tokens of b that see j, g: query heads of K/V head h
- * with the lse that ring_paged_attention_fwd returned for the same arguments (rows of lse = -inf add nothing).
+ * with the lse that ring_paged_attention_fwd returned for the same arguments (rows of lse = -inf, those that see nothing, add nothing;
+ * a row whose query or lse is NaN makes the places that it sees NaN, and no others).  Of ranks that each hold a part of the cache,
+ * every one needs the merged lse.
  * Every place is added to by one thread in a fixed order: the result does not depend on timing.  Asynchronous on `stream`.
  */
 int ring_paged_weights(const Ring_paged_params* params);

@@ -272,9 +272,13 @@ struct WeightsPlan {
     int64_t bytes() const { return part_bytes + cut_bytes; }
 };
 
-// Which form, by the query rows per K/V head.  Microseconds for 16 sequences of 8192 places, 8 K/V heads, D = 128, bf16 (rows form
-// holding 8 rows / 32 rows in registers, chunk form): 8 rows 59 / 76 / 133, 16 rows 99 / 76 / 134, 32 rows 155 / 78 / 134,
-// 40 rows 184 / 189 / 140, 64 rows 276 / 214 / 135.
+// Which form, by the query rows per K/V head.  Microseconds for 16 sequences of 8192 places, 8 K/V heads, bf16 (rows form holding 8 / 16 /
+// 32 rows in registers, chunk form):
+//   D = 128    8 rows 59 / 66 / 77 / 135    16 rows 97 / 67 / 77 / 136    24 rows 124 / 133 / 78 / 136    32 rows 151 / 141 / 79 / 136
+//             40 rows 178 / 181 / 190 / 136    64 rows 262 / 239 / 211 / 136
+//   D = 64     8 rows 38 / 45 / 58 / 133    16 rows 54 / 45 / 58 / 133    24 rows 67 / 72 / 58 / 133    32 rows 80 / 73 / 58 / 133
+//             40 rows 94 / 95 / 111 / 133    64 rows 135 / 120 / 116 / 133
+// One rule for both, although at D = 64 the rows forms stay ahead to about 64 rows.
 WeightsPlan weights_plan(const Ring_paged_params& p, int sm_count) {
     WeightsPlan r;
     const int64_t group = p.heads / p.kv_heads, rows = max_new_of(p) * group;
@@ -454,7 +458,8 @@ int ring_paged_weights(const Ring_paged_params* params) {
     a.unit_rows = 1 << 30;  // one unit holds all rows of its sequence
     a.unit_shift = 30;
     a.many_tiles = plan.chunk;
-    // in blocks.  1024 tokens over 8192 places: 102.4 / 99.2 / 98.7 us with 1 / 2 / 3; 16 single tokens (rows form): 36.1 / 36.8 / 37.6
+    // in blocks, from one case of each form: 1024 tokens over 8192 places 102.4 / 99.2 / 98.7 us with 1 / 2 / 3, 16 single tokens (rows
+    // form) 36.1 / 36.8 / 37.6
     a.start_cost = plan.chunk ? 3 : 1;
     a.min_blocks = a.start_cost + 1;
     cudaStream_t stream = static_cast<cudaStream_t>(p.stream);

@@ -14,7 +14,8 @@
 //
 // Measured: 2048 tokens over 32768 places, 32 / 8 heads, D = 128, bf16: 1.04 ms in a steady loop (1.03 PFLOP/s, 0.61 of the measured
 // cuBLAS burst rate; 0.87 ms, 1.22 PFLOP/s from idle), about 3 thousand clocks a block of 2 x 128 rows by 128 places as in the block kernel,
-// bound by its S-buffer chain.  4 chunks of 130-515 tokens over 1500-6001 places, 16 heads: 114 us; a quarter of its rows are
+// bound by its S-buffer chain.  At D = 64 the same takes 0.74 ms (0.67 PFLOP/s; its exponentials need 0.46 ms of the MUFU).  With a window of
+// 4096 + 4: 160 us at D = 128, 143 at 64.  4 chunks of 130-515 tokens over 1500-6001 places, 16 heads: 114 us; a quarter of its rows are
 // padding of the last tiles and joining the cut units takes 14 us.
 #pragma once
 
@@ -99,7 +100,8 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     constexpr int kTileBytes = T::kTileBytes;
     constexpr int kBoxBytes = T::kBoxBytes;
     constexpr int kBoxes = T::kBoxesPerTile;
-    // the producers walk the plan too: more registers than in the block kernel, or they spill
+    // The block kernel's split, although every warp follows the plan here: ptxas spills 216 bytes a thread. With 208 / 88 the softmax
+    // spills in its main loop (2048 tokens over 32768 places: 1341 us against 1071 at the time).
     constexpr int kSoftmaxRegs = 216, kProducerRegs = 72;
     static_assert(256 * kSoftmaxRegs + 128 * kProducerRegs <= 384 * 168, "what the CTA was launched with");
     constexpr uint32_t kIdescQK = umma_idesc_f16(128, BN, false, false, T::kIsBf16);
@@ -268,7 +270,7 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                         __syncwarp();
                     }
                 }
-            count_segment();
+                count_segment();
                 g = plan_next<U>(a, share, g);
             } while (ok && g.valid);
         } else if (warp == T::kMmaWarp) {
@@ -445,6 +447,8 @@ ring_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                         m_run = mx;
                     }
                     const float nms = (m_run == -INFINITY) ? 0.f : -m_run * c;
+                    // all on the MUFU: a quarter on the FMA pipe at head dimension 64, as in the block kernel, is not tried here; it would have
+                    // to be ex2_poly2's exact form, because whole rows may be hidden and a NaN score has to stay visible
                     float a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
 #pragma unroll
                     for (int v = 0; v < 128; v += 4) {

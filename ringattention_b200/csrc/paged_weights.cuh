@@ -5,14 +5,16 @@
 // Rows form (few rows: decoding): bound by reading K once.  The few-rows attention kernel's pipeline without V; the
 // places are the M side of mma.sync m16n8k16 and the query rows the N side, so 8 rows cost one instruction per 16 places.
 //
-// Chunk form (many rows): two 128 x 128 x D products per 128 query rows and 256 places, then 32768 exponentials and their sums.  The
-// MUFU does 16 exponentials a clock: 2048 clocks against 1024 of tensor time at D = 128, so the exponentials bound it.  S^T = K Q^T
-// with the places as TMEM lanes: a thread owns one place, its sum over the columns stays in a register, nothing crosses threads.
+// Chunk form (many rows): two 128 x 128 x D products per 128 query rows and 256 places, then 32768 exponentials and their sums: at 16 a
+// clock 2048 clocks of the MUFU against 1024 of tensor time at D = 128.  A quarter of the exponentials goes to the FMA pipe, which
+// leaves the MUFU 1536.  S^T = K Q^T with the places as TMEM lanes: a thread owns one place, its sum over the columns stays in a
+// register, nothing crosses threads.
 //
 // Measured: rows form, 16 sequences of 500 to 8192 places, 8 K/V heads, group 4, D = 128, one token: 36 us, 4.1 TB/s (launch, plan and the
-// last steps are a third of it).  Chunk form, 1024 tokens over 8192 places, 32 / 8 heads, D = 128: 99 us, about 2500 clocks a block
-// against the 2048 of the exponentials; moving a quarter of them to the FMA pipe took
-// 105 us to 102, half to 107.
+// last steps are a third of it).  Chunk form, 1024 tokens over 8192 places, 32 / 8 heads: 99.7 us at D = 128, 95.5 at 64 (57.7 and 55.0 with
+// a window of 2048 + 4); all exponentials on the MUFU cost 3 us more, half of them on the FMA pipe 5.  No pipe is the limit (MUFU 48 %, tensor
+// 32 % of the active clocks, issue slots 43 %): of the 171 thousand clocks a CTA is active, 53 blocks of about 2500 take 132, unit starts and
+// the plan the rest, and the busiest CTA is active for 189.
 #pragma once
 
 #include <cstdint>
