@@ -428,7 +428,8 @@ ring_block_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __gr
                 if (ok) tcgen05_fence_after_thread_sync();
             }
             if (ok) {
-                const bool have = (nblk > 0) && (l_run > 0.f);
+                // (at D = 64 the polynomial gives 2^-126 for a hidden score: a row that sees nothing has a sum, but no maximum)
+                const bool have = (nblk > 0) && (l_run > 0.f) && !(D == 64 && m_run == -INFINITY);
                 float w_new = have ? 1.f / l_run : 0.f;  // factor applied to the accumulator in TMEM
                 float lse_new = have ? m_run * a.scale + logf(l_run) : -INFINITY;
                 float w_old = 0.f;

@@ -468,7 +468,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 // 2^x for a pair of values on the FMA pipe instead of the MUFU: n = round(x) by the magic-number add, 2^(x - n) by a
 // degree-4 minimax polynomial on [-0.5, 0.5] (relative error < 3e-6), n added into the exponent field.
-// x is clamped below at -126 (the result, 2^-126, is zero where P is rounded to 16 bits) and must be below 127.
+// x is clamped below at -126 (the result, 2^-126, vanishes beside any p of a row that sees something) and must be below 127.
 // kExact, for sums that are returned: -inf gives 0 and NaN gives NaN.  The clamp is at -127 and lets NaN through; n goes in as a
 // factor whose bits are n + 127 in the exponent field, which for n = -127 is 0.f, and NaN times anything stays NaN.
 template <bool kExact = false>

@@ -69,6 +69,27 @@ def test_bf16_block_vs_oracle(shape, causal, offs):
     _check(o.cpu().numpy(), lse.cpu().numpy(), want_o, want_l, vmax, f"bf16 block {shape} causal={causal}")
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("hidden", [1, 64, 200, 300])
+def test_bf16_rows_that_see_nothing_are_zero(D, hidden):
+    """Keys that begin behind the first queries: those rows are exactly 0 with lse -inf, the others as the oracle has them."""
+    import torch
+    import ringattention_b200 as ra
+    B, H, S = 1, 2, 384
+    q, k, v = (synthetic.make_shard(x, 73, B, H, D, off, S) for x, off in (("q", 0), ("k", hidden), ("v", hidden)))
+    (tq, bq), (tk, bk), (tv, bv) = _bf16(q), _bf16(k), _bf16(v)
+    o = torch.full((B, H, S, D), float("nan"), device="cuda")
+    lse = torch.full((B, H, S), float("nan"), device="cuda")
+    ra.attention_block_fwd(tq, tk, tv, o, lse, softmax_scale=D ** -0.5, causal=True, q_off=0, k_off=hidden)
+    assert ra.device_status() == 0
+    assert bool((o[:, :, :hidden] == 0).all()) and bool(torch.isneginf(lse[:, :, :hidden]).all())
+    want_o, want_l = oracle.attention_fwd(bq, bk, bv, D ** -0.5, causal=True, q_off=0, k_off=hidden)
+    # rows of few keys: each p is off by half a step (2^-8 of it) and they sum to 1; 2^-12 for the 32-bit arithmetic
+    vmax = float(np.abs(oracle.bf16_bits_to_f32(bv)).max())
+    assert np.abs(o.cpu().numpy() - want_o).max() <= (2.0 ** -8 + 2.0 ** -12) * vmax
+    assert np.abs(lse.cpu().numpy()[:, :, hidden:] - want_l[:, :, hidden:]).max() <= TOL_LSE
+
+
 @pytest.mark.parametrize("merge_mode", [0, 1], ids=["merge-kernel", "fused-epilogue"])
 def test_bf16_virtual_ring_causal(merge_mode):
     """Three virtual ranks on one GPU, causal, bf16: the exchange, both merge forms and the block kernel's bf16 path."""
