@@ -288,7 +288,7 @@ typedef struct Ring_paged_params {
     const int* cu_seqlens; /* or NULL */
     int tokens;
     int max_new;
-    /* queries: attention and weights.  q, out [tokens, heads, dim] by strides, lse [tokens, heads] fp32 contiguous */
+    /* queries: attention and weights.  q, out [tokens, heads, dim] by strides (out's rows apart), lse [tokens, heads] fp32 contiguous */
     const void* q;
     int64_t q_token_stride, q_head_stride;
     int heads; /* a multiple of kv_heads: query head x reads K/V head x / (heads / kv_heads) */
@@ -304,7 +304,7 @@ typedef struct Ring_paged_params {
     const void* k_new;
     const void* v_new;
     int64_t k_new_token_stride, k_new_head_stride, v_new_token_stride, v_new_head_stride;
-    /* accumulated attention weight of every place, fp32 [batch, kv_heads, weights_len] by strides, places contiguous */
+    /* accumulated attention weight of every place, fp32 [batch, kv_heads, weights_len] by strides, places contiguous, rows apart */
     float* weights;
     int64_t weights_batch_stride, weights_head_stride;
     int weights_len; /* >= max_pages * page_size */

@@ -86,6 +86,10 @@ int check_tokens(const Ring_paged_params& p) {
 int check_weights(const Ring_paged_params& p) {
     PAGED_REQUIRE(p.weights_len >= static_cast<int64_t>(p.max_pages) * p.page_size, "weights_len must be at least max_pages * page_size");
     PAGED_REQUIRE(p.weights_batch_stride >= 0 && p.weights_head_stride >= 0, "weights strides must not be negative");
+    // rows are added to without atomics: two of them in one memory would lose sums
+    const int64_t places = static_cast<int64_t>(p.max_pages) * p.page_size;
+    PAGED_REQUIRE((p.batch == 1 || p.weights_batch_stride >= places) && (p.kv_heads == 1 || p.weights_head_stride >= places),
+                  "rows of weights overlap");
     return RING_OK;
 }
 
@@ -409,6 +413,7 @@ int ring_paged_attention_fwd(const Ring_paged_params* params) {
     const int out_unit = p.out_fp32 ? 3 : 7;
     PAGED_REQUIRE(((p.out_token_stride | p.out_head_stride) & out_unit) == 0 && p.out_token_stride >= 0 && p.out_head_stride >= 0,
                   "out strides must be non-negative multiples of 16 bytes");
+    PAGED_REQUIRE((p.tokens == 1 || p.out_token_stride >= p.dim) && (p.heads == 1 || p.out_head_stride >= p.dim), "rows of out overlap");
     DeviceState* st = nullptr;
     if ((rc = device_state(&st))) return rc;
     const AttentionPlan plan = attention_plan(p, st->sm_count);
@@ -488,6 +493,8 @@ int ring_paged_evict(const Ring_evict_params* params) {
     PAGED_REQUIRE(p.new_weights_len <= (1 << 30) && p.budget <= (1 << 30), "budget and new_weights_len must not exceed 2^30");
     PAGED_REQUIRE(p.weights_batch_stride >= 0 && p.weights_head_stride >= 0 && p.new_weights_batch_stride >= 0 &&
                       p.new_weights_head_stride >= 0, "weights strides must not be negative");
+    PAGED_REQUIRE((p.batch == 1 || p.new_weights_batch_stride >= p.new_weights_len) &&
+                      (p.kv_heads == 1 || p.new_weights_head_stride >= p.new_weights_len), "rows of new_weights overlap");
     ring::PagedEvictArgs e;
     cache_args(p, &e.a);
     e.a.weights = const_cast<float*>(p.weights);

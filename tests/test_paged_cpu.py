@@ -106,6 +106,18 @@ def test_evict_refuses(lib, kw, needle):
     assert needle in lib.ring_last_error_string().decode()
 
 
+@pytest.mark.parametrize("fn,kw,needle", [
+    ("ring_paged_append", dict(weights_batch_stride=0), "weights overlap"), ("ring_paged_append", dict(weights_head_stride=63), "weights overlap"),
+    ("ring_paged_weights", dict(weights_batch_stride=63), "weights overlap"), ("ring_paged_weights", dict(weights_head_stride=0), "weights overlap"),
+    ("ring_paged_attention_fwd", dict(out_token_stride=0), "out overlap"), ("ring_paged_attention_fwd", dict(out_head_stride=56), "out overlap"),
+    ("ring_paged_evict", dict(new_weights_batch_stride=0), "new_weights overlap"), ("ring_paged_evict", dict(new_weights_head_stride=31), "new_weights overlap"),
+])
+def test_results_in_one_memory_are_refused(lib, fn, kw, needle):
+    p = evict(**kw) if fn == "ring_paged_evict" else paged(**kw)
+    assert getattr(lib, fn)(ctypes.byref(p)) == _lib.RING_ERR_INVALID_ARGUMENT
+    assert needle in lib.ring_last_error_string().decode()
+
+
 def test_null_params_and_workspace(lib):
     for fn in ("ring_paged_append", "ring_paged_attention_fwd", "ring_paged_weights", "ring_paged_evict", "ring_paged_attention_workspace",
                "ring_paged_weights_workspace"):
